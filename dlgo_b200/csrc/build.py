@@ -57,9 +57,11 @@ LIBRARIES: Dict[str, List[str]] = {
     "mlstm": ["mlstm.cu"],
     "rglru": ["rglru.cu"],
     "rglru_tc": ["rglru_tc.cu"],
+    "cache_e4m3": ["cache_e4m3.cu"],
+    "attention_decode_e4m3": ["attention_decode_e4m3.cu"],
 }
 _HEADERS = ["common.cuh", "attention_noalloc.h", "attention_combine.cuh", "attention_decode_tiles.cuh", "tcgen05.cuh",
-            "async_copy.cuh", "ssd.cuh", "ssd_state.cuh"]
+            "async_copy.cuh", "ssd.cuh", "ssd_state.cuh", "e4m3.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BASE_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]

@@ -1452,6 +1452,185 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, token_p
     _check(st, "rope_append")
 
 
+# ------------------------------------------------------------ the 8-bit cache
+# A key's or a value's row of one head is kept as e4m3 numbers with one power of two:
+#   e = the smallest whole number with max |x| <= 448 * 2^e, kept within [-119, 119];   scale byte = e + 127
+#   stored = x / 2^e, clamped to +-448, to the nearest e4m3 number (ties to even);       value = stored * 2^e
+# Pages of 64 positions: keys and values [pages, kv heads, 64, head size] torch.float8_e4m3fn, scale bytes
+# [pages, kv heads, 64] torch.uint8.  bfloat16 holds every value exactly.
+E4M3_PAGE = 64
+
+
+def e4m3_takes(head_dim: int, page_size: int) -> bool:
+    """Whether the 8-bit cache's kernels take heads and pages of these sizes."""
+    return head_dim in (64, 128) and page_size == E4M3_PAGE
+
+
+def _check_e4m3(what: str, kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor, vscales: torch.Tensor,
+                page_table: torch.Tensor, num_kv_heads: Optional[int] = None, head_dim: Optional[int] = None) -> None:
+    """The shapes of the 8-bit cache's tensors fit one another and the given heads."""
+    if kpages.dim() != 4 or not e4m3_takes(kpages.shape[3], kpages.shape[2]) or kpages.shape != vpages.shape:
+        raise KernelError(f"{what}: keys and values must be [pages, kv heads, 64, 64 or 128], are {tuple(kpages.shape)} and {tuple(vpages.shape)}")
+    if kscales.shape != kpages.shape[:3] or vscales.shape != kpages.shape[:3]:
+        raise KernelError(f"{what}: a scale byte per row: {tuple(kpages.shape[:3])}, not {tuple(kscales.shape)} and {tuple(vscales.shape)}")
+    if page_table.dim() != 2 or page_table.numel() == 0 or kpages.shape[0] == 0:
+        raise KernelError(f"{what}: the page table must be [slots, pages per sequence] and the cache hold a page")
+    if num_kv_heads is not None and (num_kv_heads != kpages.shape[1] or head_dim != kpages.shape[3]):
+        raise KernelError(f"{what}: the cache's pages do not fit {num_kv_heads} heads of {head_dim}")
+
+
+def _need_e4m3(what: str, here: torch.Tensor, *tensors: tuple) -> None:
+    """Every (name, tensor, type) is contiguous, of that type and on ``here``'s GPU."""
+    for name, t, dt in tensors:
+        _need(t, dt, f"{what}: {name}")
+        if t.device != here.device:
+            raise KernelError(f"{what}: {name} lies on {t.device}, not on {here.device}")
+
+
+def _need_rows(what: str, name: str, t: torch.Tensor, rows: int, cols: int) -> None:
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols or t.stride(1) != 1:
+        raise KernelError(f"{what}: {name} must be 2-D with {rows} rows and {cols} columns next to one another")
+
+
+_E8, _U8, _I32, _F32T = torch.float8_e4m3fn, torch.uint8, torch.int32, torch.float32
+
+
+def _on_device_of(fn):
+    """Run with the first argument's device current, so that the launch goes to that device's current stream."""
+    @functools.wraps(fn)
+    def call(first: torch.Tensor, *args, **kwargs):
+        if not first.is_cuda or first.device.index == torch._C._cuda_getDevice():
+            return fn(first, *args, **kwargs)
+        with torch.cuda.device(first.device):
+            return fn(first, *args, **kwargs)
+    return call
+
+
+@_on_device_of
+def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, token_pos: torch.Tensor, token_seq: torch.Tensor,
+                     seq_slot: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor, vscales: torch.Tensor,
+                     page_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, rotary_dim: int,
+                     interleaved: bool = False, write_cache: bool = True, clear: bool = False) -> torch.Tensor:
+    """Rotate the query and key heads of ``qkv`` [tokens, q | k | v columns] (fp32 or bfloat16) at their tokens' positions in
+    fp32, store keys and values in the 8-bit pages of those positions, and return the queries [tokens, heads * head_dim] in
+    bfloat16.  ``cos`` / ``sin`` [positions, rotary_dim / 2] fp32: the first ``rotary_dim`` numbers of a head are rotated (0: none;
+    the tables are then not read), in pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1).  ``write_cache`` False:
+    queries only (a layer that reads another's cache).  ``clear`` (fp32): zeros are left where ``qkv`` was read.  A position
+    without a page is not written (:func:`check_device_errors` reports it).  Two tokens of one position in one call: either may
+    be the one that stays."""
+    what = "rope_append_e4m3"
+    if num_heads <= 0 or num_kv_heads <= 0:
+        raise KernelError(f"{what}: head counts must be positive")
+    T, cols = qkv.shape[0], (num_heads + 2 * num_kv_heads) * head_dim
+    _need_rows(what, "qkv", qkv, T, cols)
+    code = dtype_code(qkv.dtype)
+    if clear and code != F32:
+        raise KernelError(f"{what}: only an fp32 sum can be cleared")
+    _check_e4m3(what, kpages, vpages, kscales, vscales, page_table, num_kv_heads, head_dim)
+    if token_pos.numel() < T or token_seq.numel() < T or seq_slot.numel() == 0:
+        raise KernelError(f"{what}: a position and a sequence per token, and a slot per sequence")
+    if not 0 <= rotary_dim <= head_dim or rotary_dim % 2:
+        raise KernelError(f"{what}: rotary_dim must be even and no more than {head_dim}")
+    if rotary_dim and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != rotary_dim // 2 or cos.shape[0] == 0):
+        raise KernelError(f"{what}: cos and sin must be [positions, rotary_dim / 2]")
+    if not qkv.is_cuda:
+        raise KernelError(f"{what}: qkv must live on the GPU (there is no CPU path)")
+    _need_e4m3(what, qkv, ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
+               ("page_table", page_table, _I32), ("cos", cos, _F32T), ("sin", sin, _F32T), ("token_pos", token_pos, _I32),
+               ("token_seq", token_seq, _I32), ("seq_slot", seq_slot, _I32))
+    q = torch.empty((T, num_heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
+    st = _lib("cache_e4m3").dlgo_write_e4m3(
+        _ptr(qkv), _i(code), _i(T), _i(qkv.stride(0) if T > 1 else cols), _ptr(cos), _ptr(sin), _i(cos.shape[0] if rotary_dim else 0),
+        _ptr(token_pos), _ptr(token_seq), _ptr(seq_slot), _ptr(page_table), _i(page_table.shape[0]), _i(page_table.shape[1]), _ptr(kpages),
+        _ptr(vpages), _ptr(kscales), _ptr(vscales), _i(kpages.shape[0]), _ptr(q), _i(num_heads), _i(num_kv_heads), _i(head_dim),
+        _i(rotary_dim), _i(1 if interleaved else 0), _i(1 if write_cache else 0), _i(1 if clear else 0), _stream())
+    _check(st, "rope_append_e4m3", 1 if T > 0 else 0)
+    return q
+
+
+@_on_device_of
+def read_pages_e4m3(kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor, vscales: torch.Tensor, page_table: torch.Tensor,
+                    pages: torch.Tensor, keys: Optional[torch.Tensor] = None, values: Optional[torch.Tensor] = None) -> tuple:
+    """Pages of the 8-bit cache as bfloat16 (exact): ``pages`` [n, 3] int32 lists (slot, page of its sequence, rows to read);
+    returns (keys, values), each [n, kv heads, 64, head_dim], rows beyond the given number as zeros (a page that the table does
+    not have likewise).  ``keys`` / ``values``: buffers of that shape to fill instead of new ones."""
+    what = "read_pages_e4m3"
+    _check_e4m3(what, kpages, vpages, kscales, vscales, page_table)
+    if pages.dim() != 2 or pages.shape[1] != 3:
+        raise KernelError(f"{what}: pages must be [n, 3]: slot, page of its sequence, rows")
+    shape = (pages.shape[0],) + tuple(kpages.shape[1:])
+    for n, t in (("keys", keys), ("values", values)):
+        if t is not None and tuple(t.shape) != shape:
+            raise KernelError(f"{what}: {n} must be {shape}, is {tuple(t.shape)}")
+    keys = torch.empty(shape, dtype=torch.bfloat16, device=kpages.device) if keys is None else keys
+    values = torch.empty(shape, dtype=torch.bfloat16, device=kpages.device) if values is None else values
+    _need_e4m3(what, kpages, ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
+               ("page_table", page_table, _I32), ("pages", pages, _I32), ("keys", keys, torch.bfloat16), ("values", values, torch.bfloat16))
+    st = _lib("cache_e4m3").dlgo_read_e4m3(
+        _ptr(kpages), _ptr(vpages), _ptr(kscales), _ptr(vscales), _i(kpages.shape[0]), _ptr(page_table), _i(page_table.shape[0]),
+        _i(page_table.shape[1]), _ptr(pages), _i(pages.shape[0]), _ptr(keys), _ptr(values), _i(kpages.shape[1]), _i(kpages.shape[3]),
+        _stream())
+    _check(st, "read_pages_e4m3", 1 if pages.shape[0] else 0)
+    return keys, values
+
+
+def attention_decode_e4m3_scratch(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Floats of scratch of :func:`attention_decode_e4m3`, whatever the number of sequences."""
+    return int(_e4m3_scratch_fn()(_i(num_heads), _i(num_kv_heads), _i(head_dim)))
+
+
+@functools.lru_cache(maxsize=None)
+def _e4m3_scratch_fn():
+    fn = _lib("attention_decode_e4m3").dlgo_attention_decode_e4m3_scratch
+    fn.restype = ctypes.c_longlong
+    return fn
+
+
+@_on_device_of
+def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor, vscales: torch.Tensor,
+                          page_table: torch.Tensor, seq_slot: torch.Tensor, token_pos: torch.Tensor, num_heads: int, num_kv_heads: int,
+                          head_dim: int, scale: float, window: int = 0, sink: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None, scratch: Optional[torch.Tensor] = None,
+                          tickets: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over its rows of the 8-bit cache (its own key and value, at ``token_pos``,
+    included): ``q`` [sequences, heads * head_dim] bfloat16 -> [sequences, heads * head_dim] bfloat16.  ``window``: as the other
+    attention kernels take it (0: every key; w: keys t > pos - w; -c: chunks of c positions).  ``sink`` [heads] joins the
+    denominator.  A position of -1 sees nothing and gives zeros.  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
+    ``tickets`` (a zero int32 per sequence and chunk of 8 heads of a kv head, left zero) are made here when not given; given ones
+    belong to one launch at a time."""
+    what = "attention_decode_e4m3"
+    if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
+        raise KernelError(f"{what}: num_heads must be a multiple of num_kv_heads")
+    B, cols = q.shape[0], num_heads * head_dim
+    _check_e4m3(what, kpages, vpages, kscales, vscales, page_table, num_kv_heads, head_dim)
+    _need_rows(what, "q", q, B, cols)
+    if out is None:
+        out = torch.empty((B, cols), dtype=torch.bfloat16, device=q.device)
+    _need_rows(what, "out", out, B, cols)
+    if seq_slot.numel() < B or token_pos.numel() < B:
+        raise KernelError(f"{what}: a slot and a position per sequence")
+    if sink is not None and sink.numel() != num_heads:
+        raise KernelError("a sink is one number per query head")
+    if not q.is_cuda or not out.device == q.device or q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise KernelError(f"{what}: q and out must be bfloat16 and live on one GPU (there is no CPU path)")
+    floats = attention_decode_e4m3_scratch(num_heads, num_kv_heads, head_dim)
+    n_tickets = B * num_kv_heads * ((num_heads // num_kv_heads + 7) // 8)
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if scratch is None else scratch
+    tickets = torch.zeros(n_tickets, dtype=torch.int32, device=q.device) if tickets is None else tickets
+    if scratch.numel() < floats or tickets.numel() < n_tickets:
+        raise KernelError(f"{what}: {floats} floats of scratch and {n_tickets} tickets are needed")
+    _need_e4m3(what, q, ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
+               ("page_table", page_table, _I32), ("seq_slot", seq_slot, _I32), ("token_pos", token_pos, _I32),
+               ("scratch", scratch, _F32T), ("tickets", tickets, _I32), *((("sink", sink, _F32T),) if sink is not None else ()))
+    st = _lib("attention_decode_e4m3").dlgo_attention_decode_e4m3(
+        _ptr(q), _i(B), _i(q.stride(0) if B > 1 else cols), _ptr(kpages), _ptr(vpages), _ptr(kscales), _ptr(vscales), _i(kpages.shape[0]),
+        _ptr(page_table), _i(page_table.shape[0]), _i(page_table.shape[1]), _ptr(seq_slot), _ptr(token_pos), _ptr(out),
+        _i(out.stride(0) if B > 1 else cols), _i(num_heads), _i(num_kv_heads), _i(head_dim), _i(window), _f(scale), _ptr(sink), _ptr(scratch),
+        _ptr(tickets), _stream())
+    _check(st, "attention_decode_e4m3", 1 if B > 0 else 0)
+    return out
+
+
 # ------------------------------------------- head norm + rotation from frequencies + append
 def headnorm_rope_append(proj: torch.Tensor, bias: Optional[torch.Tensor], w_q: Optional[torch.Tensor],
                          w_k: Optional[torch.Tensor], eps: float, freq: Optional[torch.Tensor], rotary_dim: int,
@@ -2122,7 +2301,7 @@ def check_device_errors() -> None:
         if v != 0:
             raise KernelError("a token's position had no page in the cache's table (persistent decode kernel)")
     for lib, fn in (("rope_append", "dlgo_rope_append_error"), ("headnorm_rope", "dlgo_headnorm_rope_error"),
-                    ("wholenorm_append", "dlgo_wholenorm_append_error"),
+                    ("wholenorm_append", "dlgo_wholenorm_append_error"), ("cache_e4m3", "dlgo_cache_e4m3_error"),
                     ("attention_decode_mma", "dlgo_attention_decode_mma_error")):
         if lib in build._loaded and getattr(build._loaded[lib], fn)() != 0:
             raise KernelError("a token's position had no page in the cache's table: its keys and values were not "
