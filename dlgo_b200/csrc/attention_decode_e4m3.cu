@@ -6,22 +6,25 @@
 // v_j = V_j 2^b_j, K and V being the stored e4m3 numbers, which float16 holds exactly:
 //
 //   s_j = (q / 2^c . K_j) * (scale log2(e) 2^c 2^a_j)         c per query row, so that its largest number lies in [2^14, 2^15)
-//   t_j = s_j + b_j,   m = max s_j,   n = max t_j
-//   l = sum_j 2^(s_j - m),   O = sum_j 2^(t_j - n + 15) V_j,   out = O 2^(n - 15 - m) / l
+//   p_j = 2^(s_j - m),   w_j = p_j 2^(b_j - B) 2^f,   l = sum_j p_j,   O = sum_j w_j V_j,   out = O 2^(B - f) / l
 //
 // The queries lose nothing in float16 but what lies 2^29 below a row's largest number.  The weights of the values carry the
-// rows' powers, so they get a running maximum of their own (a row of small values may hold all of the softmax's weight);
-// up to 2^15 they have 11 bits down to 2^-29 of the largest.
+// rows' powers, so they are scaled apart from the softmax (a row of small values may hold all of its weight): B is the
+// largest power among the values, 2^f brings the largest weight to 2^10.  Both references, m and N = m + B - f, follow the
+// maxima lazily: only when a p_j passes 2^8 or a w_j 2^15 are they set anew (a vote per tile) and the sums rescaled.  A
+// weight in float16 has 11 bits down to 2^-24 of the largest, and its last bit at 2^-34.
 //
-// Bound by the rows, which are read once.  A step has one query row per head, so up to eight query heads of a kv head are the
-// rows of the 16-row MMA tile; converting the rows (an instruction for two numbers) and the scores' arithmetic cost about
-// half of what the SM can issue while memory streams.  Nothing goes through shared memory on the way in: the k index of an
-// MMA may be any permutation of a head's numbers as long as q and k agree, and so may the order of the output's numbers and
-// of the keys.  Lane (r = lane / 4, c = lane % 4) loads 16-byte pieces of rows as they lie in the pages:
-//   scores  numbers [64 v + 16 c, + 16) of the key that is column r of an 8-key tile; a 32-bit word is one k-step's share
-//   values  numbers [r HD/8, + HD/8) of keys 8c .. 8c + 7; a byte permute pairs two keys' numbers before they are converted
-// Column 2c + e of 8-key tile j is key 8c + 2j + e of the 32: a lane's eight scores belong to eight neighbouring keys, whose
-// scale bytes are one 8-byte load.
+// Bound by the rows, which are read once; next to them by issue slots: a tile of 32 keys takes some 300 instructions, of which
+// 1 per two numbers converts e4m3 to float16.  A step has one query row per head, so the keys (of the scores) and the numbers
+// of a head (of the output) are the MMA's 16 rows and up to eight query heads of a kv head its 8 columns.  Nothing goes through
+// shared memory on the way in: the k index of an MMA may be any permutation of a head's numbers as long as q and k agree, and
+// so may the order of the keys and of the output's numbers.  Lane (r = lane / 4, c = lane % 4) loads 16-byte pieces of rows as
+// they lie in the pages:
+//   scores  numbers [64 v + 16 c, + 16) of keys 4r .. 4r + 3; a 32-bit word is a k-step's share of a key.  Key 4r + 2i + h is row
+//           r + 8h of row tile i, so the lane's scores (heads 2c, 2c + 1) belong to four neighbouring keys, whose scale bytes
+//           are one word
+//   values  numbers [r HD/8, + HD/8) of keys 8c .. 8c + 7; a byte permute pairs two keys' numbers before they are converted.  The
+//           weights reach the second MMA's layout by a transposition of 8 x 8 blocks (movmatrix)
 //
 // Work is shared evenly: the tiles (32 keys) of all sequences, one sequence after another, are numbered through, and each of
 // a kv head's blocks takes an equal run of them, as many blocks as are resident at once.  A run may hold several sequences or
@@ -69,14 +72,17 @@ __device__ __forceinline__ const int* decode_pages(const DecE8& p, int i) {
   return p.page_table + (size_t)min(max(p.seq_slot[i], 0), p.n_slots - 1) * p.max_pages;
 }
 
-// d (rows 0-7 only) += A (rows 0-7; rows 8-15 are zero) * B, float16
-__device__ __forceinline__ void mma_half_rows8(float& d0, float& d1, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  [[maybe_unused]] float x2, x3;
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %10, %10};"
-      : "+f"(d0), "+f"(d1), "=f"(x2), "=f"(x3)
-      : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(0.f));
+// d += A (16 x 16) * B (16 x 8), float16 with fp32 sums
+__device__ __forceinline__ void mma_half(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// an 8 x 8 block of 16-bit numbers transposed (lane (r, c) holds row r, columns 2c and 2c + 1)
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -91,14 +97,9 @@ __device__ __forceinline__ uint32_t bf16_word(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// byte i of eight scale bytes as the power of two, and as the exponent
-__device__ __forceinline__ float byte_power(uint2 b, int i) {
-  const uint32_t w = i < 4 ? b.x : b.y;
-  return __uint_as_float(((w >> (8 * (i & 3))) & 255u) << 23);
-}
-__device__ __forceinline__ float byte_exponent(uint2 b, int i) {
-  // (2^23 + byte as bits, less 2^23 + 127: no conversion instruction)
-  return __uint_as_float(__byte_perm(i < 4 ? b.x : b.y, 0x4B000000u, 0x7440 | (i & 3))) - 8388735.f;
+// byte k of four scale bytes as the power of two
+__device__ __forceinline__ float byte_power(uint32_t w, int k) {
+  return __uint_as_float(k < 3 ? (w << (23 - 8 * k)) & 0x7f800000u : (w >> 1) & 0x7f800000u);
 }
 
 template <int HD> struct RowPiece;                 // a lane's HD / 8 numbers of a value row
@@ -107,20 +108,22 @@ template <> struct RowPiece<128> { using T = uint4; };
 __device__ __forceinline__ uint32_t piece_word(const uint2& u, int i) { return i == 0 ? u.x : u.y; }
 __device__ __forceinline__ uint32_t piece_word(const uint4& u, int i) { return i == 0 ? u.x : (i == 1 ? u.y : (i == 2 ? u.z : u.w)); }
 
+constexpr float DE_NONE = -3e38f;    // the references before the first key
 template <int HD> struct DecState {
-  float o[HD / 8][2];
-  float m, n, l;           // maximum of s, maximum of t, this lane's share of the sum
+  float o[HD / 16][4];     // tile i: numbers r HD/8 + 2i (first two) and + 2i + 1 of heads 2c, 2c + 1
+  float m[2], n[2], l[2], f[2];      // of heads 2c, 2c + 1: m, N, this lane's share of l, 2^f
+  float unit;              // 2^-B
+  int top;                 // B + 127
 };
 
 // Tiles first_tile, first_tile + DE_WARPS, ... below n_tiles (tile i: keys [32 i, 32 i + 32) of the sequence whose pages are
-// `page_row[]`), keys in [t_begin, t_end) only.
+// `page_row[]`), keys in [t_begin, t_end) only.  row_scale: of heads 2c, 2c + 1.
 template <int HD>
 __device__ __forceinline__ void decode_tiles_e8(const DecE8& p, const int* __restrict__ page_row, int kvh, int first_tile, int n_tiles,
-                                                int t_begin, int t_end, int lane, const uint32_t (&qa)[HD / 16][2], float row_scale,
-                                                DecState<HD>& st) {
+                                                int t_begin, int t_end, int lane, const uint32_t (&qb)[HD / 16][2],
+                                                const float (&row_scale)[2], DecState<HD>& st) {
   using VP = typename RowPiece<HD>::T;
   constexpr int KP = HD / 64;          // 16-byte pieces of a lane's share of a key row
-  constexpr int NT = HD / 8;
   const int r = lane >> 2, c = lane & 3;
   for (int tile = first_tile; tile < n_tiles; tile += DE_WARPS) {
     const int t0 = tile * DE_TK;
@@ -129,13 +132,13 @@ __device__ __forceinline__ void decode_tiles_e8(const DecE8& p, const int* __res
     const bool full = t0 >= t_begin && t0 + DE_TK <= t_end;      // (warp-uniform)
     // every load of the tile is requested before any arithmetic
     uint4 ku[4][KP];
-    const uint8_t* kp = p.kpages + (row0 + 8 * (r >> 1) + (r & 1)) * HD + c * 16;
+    const uint8_t* kp = p.kpages + (row0 + 4 * r) * HD + c * 16;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int v = 0; v < KP; ++v) ku[j][v] = *reinterpret_cast<const uint4*>(kp + 2 * j * HD + v * 64);
-    const uint2 kb = *reinterpret_cast<const uint2*>(p.kscales + row0 + 8 * c);
-    const uint2 vb = *reinterpret_cast<const uint2*>(p.vscales + row0 + 8 * c);
+      for (int v = 0; v < KP; ++v) ku[k][v] = *reinterpret_cast<const uint4*>(kp + k * HD + v * 64);
+    const uint32_t kb = *reinterpret_cast<const uint32_t*>(p.kscales + row0 + 4 * r);
+    const uint32_t vb = *reinterpret_cast<const uint32_t*>(p.vscales + row0 + 4 * r);
     VP vu[8];
     const uint8_t* vp = p.vpages + (row0 + 8 * c) * HD + r * (HD / 8);
     if (full) {
@@ -149,64 +152,102 @@ __device__ __forceinline__ void decode_tiles_e8(const DecE8& p, const int* __res
         if (t >= t_begin && t < t_end) vu[k] = *reinterpret_cast<const VP*>(vp + k * HD);
       }
     }
-    float s[8], w[8];
+    float s[2][4];                     // row tile i: keys 4r + 2i (first two) and + 2i + 1, heads 2c, 2c + 1
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[2 * j] = s[2 * j + 1] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
-        const uint32_t word = piece_word(ku[j][kk >> 2], kk & 3);
-        mma_half_rows8(s[2 * j], s[2 * j + 1], qa[kk][0], qa[kk][1], e4m3_low_half2(word), e4m3_high_half2(word));
+        const uint32_t w0 = piece_word(ku[2 * i][kk >> 2], kk & 3), w1 = piece_word(ku[2 * i + 1][kk >> 2], kk & 3);
+        mma_half(s[i], e4m3_low_half2(w0), e4m3_low_half2(w1), e4m3_high_half2(w0), e4m3_high_half2(w1), qb[kk][0], qb[kk][1]);
       }
     }
-    float smax = -INFINITY, tmax = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      s[k] *= row_scale * byte_power(kb, k);
-      w[k] = s[k] + byte_exponent(vb, k);
-      if (!full) {
-        const int t = t0 + 8 * c + k;
-        if (t < t_begin || t >= t_end) s[k] = w[k] = -INFINITY;
-      }
-      smax = fmaxf(smax, s[k]);
-      tmax = fmaxf(tmax, w[k]);
-    }
-    smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, 1));
-    tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
-    smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, 2));
-    tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 2));
-    const float m_new = fmaxf(st.m, smax), n_new = fmaxf(st.n, tmax);
-    const float m_ref = m_new == -INFINITY ? 0.f : m_new;
-    const float n_ref = (n_new == -INFINITY ? 0.f : n_new) - 15.f;
-    st.l *= exp2_fast(st.m - m_ref);                 // (nothing yet: 2^-inf)
-    if (__any_sync(0xffffffffu, n_new > st.n)) {
-      const float keep = exp2_fast(st.n - 15.f - n_ref);
+    for (int k = 0; k < 4; ++k) {
+      const float power = byte_power(kb, k);
+      const int t = t0 + 4 * r + k;
+      const bool seen = full || (t >= t_begin && t < t_end);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        st.o[nt][0] *= keep;
-        st.o[nt][1] *= keep;
+      for (int e = 0; e < 2; ++e) {
+        float& x = s[k >> 1][(k & 1) * 2 + e];
+        x = seen ? x * (power * row_scale[e]) : -INFINITY;
       }
     }
-    st.m = m_new;
-    st.n = n_new;
+    float w[2][4];
+    auto weights = [&](float (&add)[2], float& most_p, float& most_w) {
+      most_p = most_w = 0.f;
+      add[0] = add[1] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      st.l += exp2_fast(s[k] - m_ref);
-      w[k] = exp2_fast(w[k] - n_ref);
+      for (int k = 0; k < 4; ++k) {
+        const int t = t0 + 4 * r + k;
+        const float power = (full || (t >= t_begin && t < t_end)) ? byte_power(vb, k) * st.unit : 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float pr = exp2_fast(s[k >> 1][(k & 1) * 2 + e] - st.m[e]);
+          float& x = w[k >> 1][(k & 1) * 2 + e];
+          add[e] += pr;
+          x = pr * power * st.f[e];
+          most_p = fmaxf(most_p, pr);
+          most_w = fmaxf(most_w, x);
+        }
+      }
+    };
+    float add[2], most_p, most_w;
+    weights(add, most_p, most_w);
+    if (__any_sync(0xffffffffu, most_p > 256.f || most_w > 32768.f)) {
+      // the references anew, at least at this tile's maxima
+      int high = 8;
+      float mx[2] = {DE_NONE, DE_NONE}, nx[2] = {DE_NONE, DE_NONE};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = t0 + 4 * r + k, byte = (int)((vb >> (8 * k)) & 255u);
+        if (full || (t >= t_begin && t < t_end)) high = max(high, byte);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = s[k >> 1][(k & 1) * 2 + e];
+          mx[e] = fmaxf(mx[e], x);
+          nx[e] = fmaxf(nx[e], x + (float)(byte - 127) - 10.f);
+        }
+      }
+      high = max(st.top, __reduce_max_sync(0xffffffffu, min(high, 246)));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], o));
+          nx[e] = fmaxf(nx[e], __shfl_xor_sync(0xffffffffu, nx[e], o));
+        }
+        const float m_new = fmaxf(st.m[e], mx[e]);
+        const float n_new = fmaxf(fmaxf(st.n[e], nx[e]), m_new + (float)(high - 127) - 126.f);
+        const float keep = exp2_fast(st.n[e] - n_new);
+        st.l[e] *= exp2_fast(st.m[e] - m_new);
+        st.m[e] = m_new;
+        st.n[e] = n_new;
+        st.f[e] = exp2_fast(m_new + (float)(high - 127) - n_new);
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          st.o[i][e] *= keep;
+          st.o[i][2 + e] *= keep;
+        }
+      }
+      st.top = high;
+      st.unit = e4m3_inverse(high);
+      weights(add, most_p, most_w);
     }
+    st.l[0] += add[0];
+    st.l[1] += add[1];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const uint32_t a0 = half2_word(w[4 * ks], w[4 * ks + 1]), a2 = half2_word(w[4 * ks + 2], w[4 * ks + 3]);
+    for (int i = 0; i < 2; ++i) {
+      // keys 8c + 2i, 8c + 2i + 4 of head r, and the ones behind them
+      const uint32_t b0 = transposed(half2_word(w[i][0], w[i][1])), b1 = transposed(half2_word(w[i][2], w[i][3]));
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {            // word i of the lane's piece: four numbers, four n-tiles
-        const uint32_t k0 = piece_word(vu[4 * ks], i), k1 = piece_word(vu[4 * ks + 1], i);
-        const uint32_t k2 = piece_word(vu[4 * ks + 2], i), k3 = piece_word(vu[4 * ks + 3], i);
+      for (int j = 0; j < HD / 32; ++j) {            // word j of the lane's piece: four numbers, two row tiles
+        const uint32_t k0 = piece_word(vu[2 * i], j), k1 = piece_word(vu[2 * i + 4], j);
+        const uint32_t k2 = piece_word(vu[2 * i + 1], j), k3 = piece_word(vu[2 * i + 5], j);
         const uint32_t p01 = __byte_perm(k0, k1, 0x5140), p23 = __byte_perm(k0, k1, 0x7362);
         const uint32_t q01 = __byte_perm(k2, k3, 0x5140), q23 = __byte_perm(k2, k3, 0x7362);
-        mma_half_rows8(st.o[4 * i][0], st.o[4 * i][1], a0, a2, e4m3_low_half2(p01), e4m3_low_half2(q01));
-        mma_half_rows8(st.o[4 * i + 1][0], st.o[4 * i + 1][1], a0, a2, e4m3_high_half2(p01), e4m3_high_half2(q01));
-        mma_half_rows8(st.o[4 * i + 2][0], st.o[4 * i + 2][1], a0, a2, e4m3_low_half2(p23), e4m3_low_half2(q23));
-        mma_half_rows8(st.o[4 * i + 3][0], st.o[4 * i + 3][1], a0, a2, e4m3_high_half2(p23), e4m3_high_half2(q23));
+        mma_half(st.o[2 * j], e4m3_low_half2(p01), e4m3_high_half2(p01), e4m3_low_half2(q01), e4m3_high_half2(q01), b0, b1);
+        mma_half(st.o[2 * j + 1], e4m3_low_half2(p23), e4m3_high_half2(p23), e4m3_low_half2(q23), e4m3_high_half2(q23), b0, b1);
       }
     }
   }
@@ -218,7 +259,7 @@ template <int HD> constexpr size_t decode_e8_smem(int B, int gm) {
 
 template <int HD>
 __global__ void __launch_bounds__(DE_THREADS, HD <= 64 ? 4 : 3) attention_decode_e4m3_kernel(DecE8 p) {
-  constexpr int NT = HD / 8, AR = HD + 4;            // AR: floats from one output row to the next in shared memory
+  constexpr int AR = HD + 4;                          // AR: floats from one output row to the next in shared memory
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int last[DE_SEGS], longest;
   pdl_launch_dependents();
@@ -278,8 +319,8 @@ __global__ void __launch_bounds__(DE_THREADS, HD <= 64 ? 4 : 3) attention_decode
       const int pos = decode_pos(p, b + s), t_begin = first_visible(pos, p.span);
       const int rebase = t_begin / DE_TK - first[b + s];        // to the sequence's own tile numbers
       // head r's query in float16, its largest number in [2^14, 2^15)
-      uint32_t qa[HD / 16][2];
-      float row_scale;
+      uint32_t qb[HD / 16][2];
+      float row_scale[2];
       {
         float x[HD / 4];
         float most = 0.f;
@@ -300,35 +341,45 @@ __global__ void __launch_bounds__(DE_THREADS, HD <= 64 ? 4 : 3) attention_decode
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const int e = min(max((int)(__float_as_uint(most) >> 23), 16), 254);
         const float down = __uint_as_float((unsigned)(268 - e) << 23);          // 2^(14 - (e - 127))
-        row_scale = __uint_as_float((unsigned)(e - 14) << 23) * p.scale_log2e;
+        const float up = __uint_as_float((unsigned)(e - 14) << 23) * p.scale_log2e;
+        row_scale[0] = __shfl_sync(0xffffffffu, up, 8 * c);
+        row_scale[1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
-          qa[kk][0] = half2_word(x[4 * kk] * down, x[4 * kk + 1] * down);
-          qa[kk][1] = half2_word(x[4 * kk + 2] * down, x[4 * kk + 3] * down);
+          qb[kk][0] = half2_word(x[4 * kk] * down, x[4 * kk + 1] * down);
+          qb[kk][1] = half2_word(x[4 * kk + 2] * down, x[4 * kk + 3] * down);
         }
       }
       DecState<HD> st;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) st.o[nt][0] = st.o[nt][1] = 0.f;
-      st.m = st.n = -INFINITY;
-      st.l = 0.f;
-      decode_tiles_e8<HD>(p, decode_pages(p, b + s), kvh,
-                          begin + rebase + ((warp - (begin - lo)) & (DE_WARPS - 1)), end + rebase, t_begin, pos + 1, lane, qa, row_scale, st);
-      st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
-      st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
-      if (r < GC) {
-        float* as = acc_s + (((size_t)s * DE_WARPS + warp) * GM + r) * AR;
-        // from now on relative to m (in two steps: the values' powers may be far from the weights')
-        const float f = st.m == -INFINITY ? 0.f : exp2_fast(0.5f * (st.n - 15.f - st.m));
+      for (int i = 0; i < HD / 16; ++i) st.o[i][0] = st.o[i][1] = st.o[i][2] = st.o[i][3] = 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {            // MMA column nt * 8 + 2c + e is number (2c + e) * HD/8 + nt of the head
-          as[(2 * c) * (HD / 8) + nt] = st.o[nt][0] * f * f;
-          as[(2 * c + 1) * (HD / 8) + nt] = st.o[nt][1] * f * f;
-        }
-        if (c == 0) {
-          float* ml = ml_s + ((s * DE_WARPS + warp) * GM + r) * 2;
-          ml[0] = st.m;
-          ml[1] = st.l;
+      for (int e = 0; e < 2; ++e) {
+        st.m[e] = st.n[e] = DE_NONE;
+        st.l[e] = 0.f;
+        st.f[e] = 1.f;
+      }
+      st.unit = 1.f;
+      st.top = 8;
+      decode_tiles_e8<HD>(p, decode_pages(p, b + s), kvh, begin + rebase + ((warp - (begin - lo)) & (DE_WARPS - 1)), end + rebase, t_begin,
+                          pos + 1, lane, qb, row_scale, st);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], o);
+        const int g = 2 * c + e;
+        if (g >= GC) continue;
+        // from now on relative to m (in two steps: the values' powers may be far from the weights')
+        float* as = acc_s + (((size_t)s * DE_WARPS + warp) * GM + g) * AR + r * (HD / 8);
+        const float f = exp2_fast(0.5f * (st.n[e] - st.m[e]));
+#pragma unroll
+        for (int i = 0; i < HD / 16; i += 2)
+          *reinterpret_cast<float4*>(as + 2 * i) = make_float4(st.o[i][e] * f * f, st.o[i][2 + e] * f * f, st.o[i + 1][e] * f * f,
+                                                               st.o[i + 1][2 + e] * f * f);
+        if (r == 0) {
+          float* ml = ml_s + ((s * DE_WARPS + warp) * GM + g) * 2;
+          ml[0] = st.m[e];
+          ml[1] = st.l[e];
         }
       }
     }
@@ -358,7 +409,7 @@ __global__ void __launch_bounds__(DE_THREADS, HD <= 64 ? 4 : 3) attention_decode
 #pragma unroll
       for (int w = 0; w < DE_WARPS; ++w) {
         const float mw = ml[w * GM * 2];
-        const float cw = mw == -INFINITY ? 0.f : exp2_fast(mw - mm);
+        const float cw = exp2_fast(mw - mm);
         const float4 u = *reinterpret_cast<const float4*>(as + w * GM * AR);
         a.x = fmaf(cw, u.x, a.x); a.y = fmaf(cw, u.y, a.y); a.z = fmaf(cw, u.z, a.z); a.w = fmaf(cw, u.w, a.w);
         ll = fmaf(cw, ml[w * GM * 2 + 1], ll);
