@@ -2287,7 +2287,8 @@ def gemm_tc_rope(x: torch.Tensor, w: torch.Tensor, qkv: torch.Tensor, pair_tile:
 def check_device_errors() -> None:
     """Raise if a kernel gave up a bounded wait on the device since the last check (synchronises)."""
     for lib, fn in (("gemm_tc", "dlgo_gemm_tc_error"), ("attention_prefill_tc", "dlgo_attention_tc_error"),
-                    ("moe_tc", "dlgo_moe_tc_error"), ("rglru_tc", "dlgo_rglru_gates_tc_error")):
+                    ("moe_tc", "dlgo_moe_tc_error"), ("rglru_tc", "dlgo_rglru_gates_tc_error"),
+                    ("attention_decode_e4m3", "dlgo_attention_decode_e4m3_error")):
         if lib in build._loaded:
             v = getattr(build._loaded[lib], fn)()
             if v != 0:
