@@ -3,18 +3,19 @@
 //
 // One new token per sequence; scores s_j = q . k_j * scale over the visible positions, softmax, weighted sum of the values
 // (models/llm/forward.go:258-278, with rows that take hd + 1 bytes instead of 2 hd).  With k_j = K_j 2^a_j and
-// v_j = V_j 2^b_j, K and V being the stored e4m3 numbers, per query head and tile of 128 keys:
+// v_j = V_j 2^b_j, K and V being the stored e4m3 numbers, per query head and tile of 128 keys (256 with heads of 64):
 //
 //   s_j = (K_j . q') * 2^a_j * (scale log2(e) 2^c)      q' = q / 2^c, its largest number in [2^7, 2^8)
-//   p_j = 2^(s_j - m),  l = sum_j p_j                   m = the running maximum of s_j, rounded up to a whole number
-//   w_j = 2^(s_j + b_j - n + 8),  O' = sum_j w_j V_j    n = the tile's maximum of s_j + b_j, rounded up: w_j <= 2^8
+//   p_j = 2^(s_j - m),  l = sum_j p_j                   m = the maximum of s_j so far of the keys that one thread sees; the
+//                                                       threads' sums meet at the sequence's end
+//   w_j = 2^(s_j + b_j - n + 8),  O' = sum_j w_j V_j    n = the tile's maximum of s_j + b_j: w_j <= 2^8
 //   O = O 2^(n_before - N) + O' 2^(n - N)               N = the running maximum of n
 //   out = O 2^(N - 8 - m) / l
 //
 // Both products have e4m3 on both sides.  The other operand enters as several e4m3 terms in columns of their own: a query as
 // x = x1 + x2 / 16, which holds a bfloat16 number whole down to 2^-22 of the row's largest (each term keeps 4 bits, and what
 // the first leaves over is at most 2^-4 of it); a weight as w1 + w2 / 16 (+ w3 / 256 where a block has four heads at most):
-// 2^-8 (2^-12) of its size, and of the tile's largest weight 2^-22 (2^-26).  The values' powers are part of the weights, so a
+// 2^-8 (2^-11, passing through float16) of its size, and of the tile's largest weight 2^-22 (2^-26).  The values' powers are part of the weights, so a
 // row of small values may hold all of the softmax's weight without a loss; and because every tile has a reference of its
 // own, neither does a long tail of small weights behind a large one.
 //
@@ -22,16 +23,20 @@
 // MMA's rows and the query heads of a kv head, times their terms, its 16 columns, so no thread touches a row: per tile
 // a thread handles one key's scores.  (With mma.sync, whose operands are at least 16 bits wide, converting the rows and the
 // scores' arithmetic took 424 instructions per 32 keys and warp: 32 sequences of 256 to 4,096 keys, heads of 128, 35.2 us.)
-//   warp 0     TMA: two pages of keys and of values per tile, and their scale bytes, into rings
-//   warp 1     tcgen05.mma: scores (keys x 16) one tile ahead, output (numbers x 16); values as the MN-major operand from the
-//              page layout [key][number], weights MN-major as the threads write them, 16 bytes a key
-//   warps 2-5  a thread per key: scores, maxima over the tile (redux and a barrier), weights; then, a thread per number of a
-//              head, the output of the tile before
-// Two such blocks share an SM (three with heads of 64), so one's chain of steps runs under the other's.
+//   warp 0     TMA, a lane per page: keys, values and scale bytes into rings
+//   warps 1, 2 tcgen05.mma: scores (128 keys x 16, once or twice); output (numbers x 16), values as the MN-major operand from the
+//              page layout [key][number], weights MN-major as the threads write them, 16 bytes a key.  (One thread for both
+//              took 3,200 clocks a tile: it was what the others waited for.)
+//   warps 3-6  a thread per key, or per two: scores, maxima over the tile (redux and a barrier), weights; then, a thread per number of
+//              a head, the output of the tile before
+// Two such blocks share an SM, so one's chain of steps runs under the other's.  The chain is what tiles of 256 keys are for with
+// heads of 64: with 128, some 300 instructions and 2,800 clocks a tile, three blocks' chains did not keep up with memory (one
+// sequence of 131,072 keys 38 us).
 //
 // Work is shared evenly: the tiles of all sequences and kv heads are numbered through, head by head and sequence by sequence,
 // and every block takes an equal run of them, as many blocks as are resident at once: all SMs stream until the end, whatever
-// the lengths.  What blocks share, at most the first and the last sequence of each, goes through scratch memory, and the block
+// the lengths.  A sequence's first tile counts twice: its queries, the end of the sequence before and the pause between them
+// cost about as much as a tile.  What blocks share, at most the first and the last sequence of each, goes through scratch memory, and the block
 // that takes a sequence's last ticket adds the parts up in the order of the blocks; nobody waits for another block.
 #include <math.h>
 
@@ -43,17 +48,18 @@ namespace dlgo {
 
 using namespace sm100;
 
-constexpr int DE_THREADS = 192;
-constexpr int DE_SOFT = 128;          // of them, warps 2-5
-constexpr int DE_TK = 128;            // keys of a tile: two pages
+constexpr int DE_THREADS = 224;
+constexpr int DE_SOFT = 128;          // of them, warps 3-6
+// halves of a tile, of 128 keys (two pages) each
+template <int HD> constexpr int de_halves = HD <= 64 ? 2 : 1;
 constexpr int DE_GM = 8;              // query heads of a kv head per block at most
-constexpr int DE_MIN_TILES = 2;       // a block's least run
-constexpr int DE_MAX_B = 512;         // sequences of a launch (their first tiles, positions and slots lie in shared memory)
-constexpr int DE_SC = 4;              // tiles whose scale bytes are on their way or in use
+constexpr int DE_MIN_RUN = 2;         // a block's least run (so that none lies within one tile)
+constexpr int DE_MAX_B = 1024;        // sequences of a launch (their first tiles, positions and slots lie in shared memory)
+constexpr int DE_BARS = 40;           // room for barriers
+constexpr int DE_SC = 3;              // tiles whose scale bytes are on their way or in use
 
-template <int HD> constexpr int de_kst = 3;                          // tiles of keys, of values in shared memory
-template <int HD> constexpr int de_vst = HD <= 64 ? 3 : 2;
-template <int HD> constexpr int de_blocks = HD <= 64 ? 3 : 2;        // blocks on an SM
+constexpr int DE_KST = 2, DE_VST = 2; // tiles of keys, of values in shared memory (16 KB each; a third of keys gains nothing)
+constexpr int DE_BLOCKS = 2;          // blocks on an SM
 
 // Set when a bounded wait ran out: the launch's results are invalid (dlgo_attention_decode_e4m3_error).
 __device__ int g_decode_e4m3_error = 0;
@@ -81,8 +87,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^x for a whole x; below -126: 0
-__device__ __forceinline__ float exp2_whole(float x) { return __int_as_float(max((int)fmaxf(x, -127.f) + 127, 0) << 23); }
 __device__ __forceinline__ uint32_t bf16_word(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -92,7 +96,23 @@ __device__ __forceinline__ float warp_max_redux(float x) {     // (a NaN does no
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// float16 pairs to e4m3, the first number in the low byte
+__device__ __forceinline__ uint32_t e4m3_of_half2(__half2 h) {
+  uint16_t q;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
+  return q;
+}
+__device__ __forceinline__ __half2 half2_of_e4m3(uint32_t pair) {
+  const uint32_t h = e4m3_low_half2(pair);
+  return *reinterpret_cast<const __half2*>(&h);
+}
 // two e4m3 numbers back as fp32
 __device__ __forceinline__ float2 e4m3_back(uint32_t pair) {
   const uint32_t h = e4m3_low_half2(pair);
@@ -129,28 +149,29 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, ui
       : "memory");
 }
 
-// A tile of the run: virtual head (kv head and chunk of its query heads), sequence, tile k of its nk.
+// A tile of the run: virtual head (kv head and chunk of its query heads), sequence, tile k of its nk, the sequence's pages from
+// there on.
 struct DecPlace {
-  int head, b, k, nk;
+  int head, b, k, nk, pages;
 };
 
 // Shared memory: rings of keys and of values, two buffers of queries and of weights, scale bytes, barriers, ... , sequences
-template <int HD> constexpr int de_off_q = (de_kst<HD> + de_vst<HD>) * DE_TK * HD;
+template <int HD> constexpr int de_off_q = (DE_KST + DE_VST) * de_halves<HD> * 128 * HD;
 template <int HD> constexpr int de_off_p = de_off_q<HD> + 2 * 16 * HD;
-template <int HD> constexpr int de_off_sc = de_off_p<HD> + 2 * 2048;
-template <int HD> constexpr int de_off_bars = de_off_sc<HD> + DE_SC * 256;
-template <int HD> constexpr int de_off_red = de_off_bars<HD> + 256;             // [2][4][2][GM] floats
-template <int HD> constexpr int de_off_misc = de_off_red<HD> + 2 * 4 * 2 * DE_GM * 4;    // row scales [2][GM], sums [4][GM], words
-template <int HD> constexpr int de_off_seq = de_off_misc<HD> + 6 * DE_GM * 4 + 64;
+template <int HD> constexpr int de_off_sc = de_off_p<HD> + 2 * de_halves<HD> * 2048;
+template <int HD> constexpr int de_off_bars = de_off_sc<HD> + DE_SC * de_halves<HD> * 256;
+template <int HD> constexpr int de_off_red = de_off_bars<HD> + DE_BARS * 8;             // [2][4][GM] floats
+template <int HD> constexpr int de_off_misc = de_off_red<HD> + 2 * 4 * DE_GM * 4;    // row scales [2][GM], maxima and sums [GM][4], words
+template <int HD> constexpr int de_off_seq = de_off_misc<HD> + 10 * DE_GM * 4 + 64;
 template <int HD> constexpr size_t de_smem(int B) { return de_off_seq<HD> + (size_t)(4 * B + 1) * 4; }
 
 template <int HD, int GM>
-__global__ void __launch_bounds__(DE_THREADS, de_blocks<HD>)
+__global__ void __launch_bounds__(DE_THREADS, DE_BLOCKS)
 attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DecE8 p) {
   constexpr int TERMS = GM <= 4 ? 3 : 2;
-  constexpr int KST = de_kst<HD>, VST = de_vst<HD>, STAGE = DE_TK * HD, PAGE_BYTES = E8_PAGE * HD;
-  constexpr uint32_t TMEM_COLS = 64, O_COL = 32;      // scores in columns 0 and 16, outputs in 32 and 48
-  constexpr int H4 = HD / 4;
+  constexpr int H = de_halves<HD>, KST = DE_KST, VST = DE_VST, STAGE = H * 128 * HD, PAGE_BYTES = E8_PAGE * HD;
+  constexpr uint32_t TMEM_COLS = 128, O_COL = 64;     // scores of two tiles in columns 0 to 63, outputs in 64 and 80
+  constexpr int H4 = HD / 4, JN = GM <= 4 ? 8 : 4;
   // the swizzled tiles want 1024-byte alignment (checked: a misaligned start ends the kernel with the error word set)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -160,28 +181,29 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
   uint8_t* k_s = smem;
   uint8_t* v_s = k_s + KST * STAGE;
   uint8_t* q_s = smem + de_off_q<HD>;                 // [2][16 rows][HD], swizzled as the keys
-  uint8_t* p_s = smem + de_off_p<HD>;                 // [2][128 keys][16]
-  uint8_t* sc_s = smem + de_off_sc<HD>;               // [DE_SC][keys 128 | values 128]
+  uint8_t* p_s = smem + de_off_p<HD>;                 // [2][H][128 keys][16]
+  uint8_t* sc_s = smem + de_off_sc<HD>;               // [DE_SC][H][keys 128 | values 128]
   uint64_t* bars = (uint64_t*)(smem + de_off_bars<HD>);
   uint64_t* kfull = bars;                // KST
-  uint64_t* kempty = bars + 3;           // KST: the scores that read these keys have completed
-  uint64_t* vfull = bars + 6;            // VST
-  uint64_t* vempty = bars + 9;           // VST: the output that read these values has completed
-  uint64_t* sc_full = bars + 12;         // DE_SC
-  uint64_t* sc_empty = bars + 16;        // DE_SC
-  uint64_t* s_full = bars + 20;          // 2: scores
-  uint64_t* s_free = bars + 22;          // 2: ... are in registers
-  uint64_t* p_full = bars + 24;          // 2: weights
-  uint64_t* o_full = bars + 26;          // 2: the output of a tile (its weights may be overwritten)
-  uint64_t* o_free = bars + 28;          // 2: ... is in registers
-  uint64_t* q_full = bars + 30;          // 2
+  uint64_t* kempty = kfull + KST;        // KST: the scores that read these keys have completed
+  uint64_t* vfull = kempty + KST;        // VST
+  uint64_t* vempty = vfull + VST;        // VST: the output that read these values has completed
+  uint64_t* sc_full = vempty + VST;      // DE_SC
+  uint64_t* sc_empty = sc_full + DE_SC;  // DE_SC
+  uint64_t* s_full = sc_empty + DE_SC;   // 2: scores
+  uint64_t* s_free = s_full + 2;         // 2: ... are in registers
+  uint64_t* p_full = s_free + 2;         // 2: weights
+  uint64_t* o_full = p_full + 2;         // 2: the output of a tile (its weights may be overwritten)
+  uint64_t* o_free = o_full + 2;         // 2: ... is in registers
+  uint64_t* q_full = o_free + 2;         // 2
+  static_assert(2 * KST + 2 * VST + 2 * DE_SC + 12 <= DE_BARS, "the barriers fit");
   float* red_s = (float*)(smem + de_off_red<HD>);
   float* fs_s = (float*)(smem + de_off_misc<HD>);     // [2][DE_GM] row scales
-  float* l_s = fs_s + 2 * DE_GM;                      // [4][DE_GM]
-  int* sums = (int*)(l_s + 4 * DE_GM);                // [6]
-  int& last = sums[6];
-  uint32_t* tmem_slot = (uint32_t*)(sums + 7);
-  volatile int* abort_flag = sums + 8;
+  float2* ml_s = (float2*)(fs_s + 2 * DE_GM);         // [DE_GM][4 warps] maximum and sum
+  int* sums = (int*)(ml_s + 4 * DE_GM);               // [8]
+  int& last = sums[8];
+  uint32_t* tmem_slot = (uint32_t*)(sums + 9);
+  volatile int* abort_flag = sums + 10;
   int* first = (int*)(smem + de_off_seq<HD>);         // [B + 1] first tile of each sequence
   const int B = p.B, G = p.Hq / p.Hkv, heads = p.Hkv * p.n_gchunks;
   int* pos_s = first + B + 1;                         // [B] last visible position
@@ -190,9 +212,11 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    for (int s = 0; s < 3; ++s) {
+    for (int s = 0; s < KST; ++s) {
       mbar_init(&kfull[s], 1);
       mbar_init(&kempty[s], 1);
+    }
+    for (int s = 0; s < VST; ++s) {
       mbar_init(&vfull[s], 1);
       mbar_init(&vempty[s], 1);
     }
@@ -214,6 +238,10 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     tma_prefetch_desc(&map_v);
     first[0] = 0;
   }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
   // the cut, from the step's own inputs (kept within the table whatever they are)
   for (int b0 = 0, sum = 0; b0 < B; b0 += DE_THREADS) {
     const int i = b0 + tid;
@@ -223,7 +251,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       pos_s[i] = pos;
       begin_s[i] = begin;
       slot_s[i] = min(max(p.seq_slot[i], 0), p.n_slots - 1);
-      n = (max(pos, 0) / E8_PAGE - begin / E8_PAGE) / 2 + 1;
+      n = (max(pos, 0) / E8_PAGE - begin / E8_PAGE) / (2 * H) + 2;         // (its first tile counts twice)
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -231,115 +259,167 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       if (lane >= o) n += up;
     }
     if (lane == 31) sums[warp] = n;
+    tc_fence_before_sync();
     __syncthreads();
     for (int k = 0; k < warp; ++k) n += sums[k];
     if (i < B) first[i + 1] = n + sum;
     for (int k = 0; k < DE_THREADS / 32; ++k) sum += sums[k];
     __syncthreads();
   }
-  const int P = first[B];
-  const long long total = (long long)heads * P;
-  const unsigned nb = (unsigned)min((long long)gridDim.x, (total + DE_MIN_TILES - 1) / DE_MIN_TILES);   // (no run is empty)
-  if (blockIdx.x >= nb) return;                       // (nothing is on its way yet)
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   pdl_launch_dependents();       // (now: a successor's block may wait for tensor memory, but never one of these behind it)
-
-  auto block_of = [&](long long tile) { return (int)(((tile + 1) * nb - 1) / total); };
-  const long long lo = blockIdx.x * total / nb, hi = (blockIdx.x + 1) * total / nb;
-  const int n_tiles = (int)(hi - lo);
-  DecPlace start;
-  start.head = (int)(lo / P);
-  {
-    const int y = (int)(lo - (long long)start.head * P);
-    int b = 0;
-    for (int step = DE_MAX_B / 2; step > 0; step >>= 1)
-      if (b + step < B && first[b + step] <= y) b += step;
-    start.b = b;
-    start.k = y - first[b];
-    start.nk = first[b + 1] - first[b];
+  const int P = first[B];
+  const long long total = (long long)heads * P;       // (counting first tiles twice)
+  const unsigned nb = (unsigned)min((long long)gridDim.x, total / DE_MIN_RUN);        // (every sequence counts two at least)
+  const bool narrow = total < 0xffffffffLL / (nb + 1);                                // (a division of 64 bits takes 100 instructions)
+  auto start_of = [&](unsigned i) { return narrow ? (long long)(i * (unsigned)total / nb) : (long long)i * total / nb; };
+  auto block_of = [&](long long x) { return (int)(narrow ? ((unsigned)(x + 1) * nb - 1) / (unsigned)total : ((x + 1) * nb - 1) / total); };
+  auto enter = [&](DecPlace& x) {                     // what a sequence's tile k follows from the sequence
+    x.nk = first[x.b + 1] - first[x.b] - 1;
+    x.pages = max(pos_s[x.b], 0) / E8_PAGE - begin_s[x.b] / E8_PAGE + 1 - 2 * H * x.k;
+  };
+  // the place that the count x falls on: tile k begins at the sequence's count 0 (k = 0) or k + 1
+  auto place = [&](long long x) {
+    DecPlace at;
+    at.head = (int)(narrow ? (unsigned)x / (unsigned)P : x / P);
+    const int y = (int)(x - (long long)at.head * P);
+    int b = -1;                                       // the last sequence whose first count is no more than y
+    for (int i = lane; i < B; i += 32) b += first[i] <= y;
+    b = __reduce_add_sync(0xffffffffu, b + 1) - 1;
+    const int u = y - first[b];
+    at.b = b;
+    at.k = u == 0 ? 0 : max(1, u - 1);
+    // A place behind the start of the sequence's last tile, and one within a sequence of two tiles, is the start of the next: two
+    // tiles one after another take less than their parts' way through memory (8 sequences of 100 to 160 keys, heads of 128,
+    // 6.3 us against 11.8).
+    const int nk = first[b + 1] - first[b] - 1;
+    if (at.k >= nk || (at.k > 0 && nk <= 2)) {
+      at.k = 0;
+      if (++at.b == B) {
+        at.b = 0;
+        ++at.head;
+      }
+    }
+    enter(at);
+    return at;
+  };
+  int n_tiles = 0;
+  DecPlace start = {0, 0, 0, 1, 1};
+  if (blockIdx.x < nb) {
+    start = place(start_of(blockIdx.x));
+    const DecPlace end = place(start_of(blockIdx.x + 1));
+    // tiles up to a place: those of the heads and sequences before it, and its k
+    n_tiles = (end.head - start.head) * (P - B) + (first[end.b] - end.b + end.k) - (first[start.b] - start.b + start.k);
   }
   auto advance = [&](DecPlace& x) {                   // to the next tile; true: of another sequence or head
+    x.pages -= 2 * H;
     if (++x.k < x.nk) return false;
     x.k = 0;
     if (++x.b == B) {
       x.b = 0;
       ++x.head;
     }
-    x.nk = first[x.b + 1] - first[x.b];
+    enter(x);
     return true;
   };
-  auto two_pages = [&](const DecPlace& x) { return begin_s[x.b] / E8_PAGE + 2 * x.k + 1 <= max(pos_s[x.b], 0) / E8_PAGE; };
-  pdl_wait();
-
+  auto pages_of = [&](const DecPlace& x) { return min(2 * H, x.pages); };
   if (warp == 0) {
-    if (elect_one()) {
-      DecPlace at = start;
-      bool ok = true;
-      for (int it = 0; ok && it < n_tiles; ++it) {
-        const int kvh = at.head / p.n_gchunks, pg = begin_s[at.b] / E8_PAGE + 2 * at.k, n = two_pages(at) ? 2 : 1;
-        const int* row = p.page_table + (size_t)slot_s[at.b] * p.max_pages + pg;
-        int rows[2];                                  // first row of each page's kv head
-        for (int j = 0; j < n; ++j) rows[j] = (min(max(row[j], 0), p.n_pages - 1) * p.Hkv + kvh) * E8_PAGE;
-        const int ks = it % KST, vs = it % VST, cs = it % DE_SC;
-        if (it >= KST) ok = mbar_wait(&kempty[ks], (it / KST - 1) & 1, abort_flag);
-        if (!ok) break;
-        mbar_expect_tx(&kfull[ks], n * PAGE_BYTES);
-        for (int j = 0; j < n; ++j) tma_load_2d(k_s + ks * STAGE + j * PAGE_BYTES, &map_k, &kfull[ks], 0, rows[j]);
-        if (it >= DE_SC) ok = mbar_wait(&sc_empty[cs], (it / DE_SC - 1) & 1, abort_flag);
-        if (!ok) break;
-        mbar_expect_tx(&sc_full[cs], n * 2 * E8_PAGE);
-        for (int j = 0; j < n; ++j) {
-          bulk_load(sc_s + cs * 256 + j * E8_PAGE, p.kscales + rows[j], E8_PAGE, &sc_full[cs]);
-          bulk_load(sc_s + cs * 256 + 128 + j * E8_PAGE, p.vscales + rows[j], E8_PAGE, &sc_full[cs]);
-        }
-        if (it >= VST) ok = mbar_wait(&vempty[vs], (it / VST - 1) & 1, abort_flag);
-        if (!ok) break;
-        mbar_expect_tx(&vfull[vs], n * PAGE_BYTES);
-        for (int j = 0; j < n; ++j) tma_load_2d(v_s + vs * STAGE + j * PAGE_BYTES, &map_v, &vfull[vs], 0, rows[j]);
+    // Lane j: page j of the tile.  Keys and scale bytes run a tile ahead of values, whose room is free only when the output
+    // before is done; page numbers another tile ahead, the first ones before the launch before this has ended.
+    DecPlace at = start;
+    const int j = lane & (2 * H - 1);
+    const bool mine = lane < 2 * H;
+    int page = 0, row = 0, n = 0, v_row, v_n;
+    auto look_up = [&]() {
+      page = p.page_table[(size_t)slot_s[at.b] * p.max_pages + begin_s[at.b] / E8_PAGE + 2 * H * at.k + min(j, pages_of(at) - 1)];
+    };
+    if (n_tiles > 0) look_up();
+    pdl_wait();
+    bool ok = true;
+    for (int it = 0; it <= n_tiles && n_tiles > 0; ++it) {
+      v_row = row;
+      v_n = n;
+      if (it < n_tiles) {
+        n = pages_of(at);
+        row = (min(max(page, 0), p.n_pages - 1) * p.Hkv + at.head / p.n_gchunks) * E8_PAGE;   // first of the kv head
         advance(at);
+        if (it + 1 < n_tiles) look_up();
+        const int cs = it % DE_SC, ks = it % KST;
+        if (it >= DE_SC) ok = mbar_wait(&sc_empty[cs], (it / DE_SC - 1) & 1, abort_flag);
+        if (ok && it >= KST) ok = mbar_wait(&kempty[ks], (it / KST - 1) & 1, abort_flag);
+        if (__any_sync(0xffffffffu, !ok)) break;
+        if (lane == 0) {
+          mbar_expect_tx(&kfull[ks], n * PAGE_BYTES);
+          mbar_expect_tx(&sc_full[cs], n * 2 * E8_PAGE);
+        }
+        __syncwarp();
+        if (mine && j < n) {
+          tma_load_2d(k_s + ks * STAGE + j * PAGE_BYTES, &map_k, &kfull[ks], 0, row);
+          uint8_t* dst = sc_s + (cs * H + j / 2) * 256 + j % 2 * E8_PAGE;
+          bulk_load(dst, p.kscales + row, E8_PAGE, &sc_full[cs]);
+          bulk_load(dst + 128, p.vscales + row, E8_PAGE, &sc_full[cs]);
+        }
+      }
+      if (it > 0) {
+        const int vi = it - 1, vs = vi % VST;
+        if (vi >= VST) ok = mbar_wait(&vempty[vs], (vi / VST - 1) & 1, abort_flag);
+        if (__any_sync(0xffffffffu, !ok)) break;
+        if (lane == 0) mbar_expect_tx(&vfull[vs], v_n * PAGE_BYTES);
+        __syncwarp();
+        if (mine && j < v_n) tma_load_2d(v_s + vs * STAGE + j * PAGE_BYTES, &map_v, &vfull[vs], 0, v_row);
       }
     }
   } else if (warp == 1) {
+    pdl_wait();
     if (elect_one()) {
-      constexpr uint32_t idesc_s = idesc_e4m3(DE_TK, 16, false), idesc_o = idesc_e4m3(HD, 16, true);
-      DecPlace ahead = start, at = start;             // the tile whose scores, whose output come next
+      constexpr uint32_t idesc = idesc_e4m3(128, 16, false);
+      DecPlace at = start;
       int seg = 0;
       bool fresh = true, ok = true;
-      auto scores = [&](int it) {
+      for (int it = 0; it < n_tiles; ++it) {
         const int ks = it % KST;
         if (fresh) ok = mbar_wait(&q_full[seg & 1], (seg >> 1) & 1, abort_flag);
         if (ok && it >= 2) ok = mbar_wait(&s_free[it & 1], ((it >> 1) - 1) & 1, abort_flag);
         if (ok) ok = mbar_wait(&kfull[ks], (it / KST) & 1, abort_flag);
-        if (!ok) return;
-        tc_fence_after_sync();
-        const uint64_t a = desc_rows<HD>(smem_u32(k_s + ks * STAGE)), b = desc_rows<HD>(smem_u32(q_s + (seg & 1) * 16 * HD));
-#pragma unroll
-        for (int k = 0; k < HD / 32; ++k) umma_e4m3(tmem_base + (it & 1) * 16, a + 2 * k, b + 2 * k, idesc_s, k != 0);
-        umma_commit(&s_full[it & 1]);
-        umma_commit(&kempty[ks]);
-        fresh = advance(ahead);
-        if (fresh) ++seg;
-      };
-      scores(0);
-      for (int it = 0; ok && it < n_tiles; ++it) {
-        if (it + 1 < n_tiles) scores(it + 1);
-        const int vs = it % VST;
-        if (ok) ok = mbar_wait(&p_full[it & 1], (it >> 1) & 1, abort_flag);
-        if (ok && it >= 2) ok = mbar_wait(&o_free[it & 1], ((it >> 1) - 1) & 1, abort_flag);
-        if (ok) ok = mbar_wait(&vfull[vs], (it / VST) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after_sync();
-        const uint64_t a = desc_rows<HD>(smem_u32(v_s + vs * STAGE)), b = desc_weights(smem_u32(p_s + (it & 1) * 2048));
-        const int steps = two_pages(at) ? 4 : 2;      // 32 keys each
-        for (int k = 0; k < steps; ++k)
-          umma_e4m3(tmem_base + O_COL + (it & 1) * 16, a + k * (32 * HD >> 4), b + k * (32 * 16 >> 4), idesc_o, k != 0);
+        const uint64_t a = desc_rows<HD>(smem_u32(k_s + ks * STAGE)), b = desc_rows<HD>(smem_u32(q_s + (seg & 1) * 16 * HD));
+        const int n = pages_of(at);
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+          if (2 * h < n) {
+#pragma unroll
+            for (int k = 0; k < HD / 32; ++k)
+              umma_e4m3(tmem_base + (it & 1) * 32 + h * 16, a + h * (128 * HD >> 4) + 2 * k, b + 2 * k, idesc, k != 0);
+          }
+        umma_commit(&s_full[it & 1]);
+        umma_commit(&kempty[ks]);
+        fresh = advance(at);
+        if (fresh) ++seg;
+      }
+    }
+  } else if (warp == 2) {
+    pdl_wait();
+    if (elect_one()) {
+      constexpr uint32_t idesc = idesc_e4m3(HD, 16, true);
+      DecPlace at = start;
+      bool ok = true;
+      for (int it = 0; it < n_tiles; ++it) {
+        const int vs = it % VST;
+        if (it >= 2) ok = mbar_wait(&o_free[it & 1], ((it >> 1) - 1) & 1, abort_flag);
+        if (ok) ok = mbar_wait(&vfull[vs], (it / VST) & 1, abort_flag);
+        if (ok) ok = mbar_wait(&p_full[it & 1], (it >> 1) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint64_t a = desc_rows<HD>(smem_u32(v_s + vs * STAGE)), b = desc_weights(smem_u32(p_s + (it & 1) * H * 2048));
+        const int n = pages_of(at);
+#pragma unroll
+        for (int j = 0; j < 2 * H; ++j)
+          if (j < n) {                                // a page: twice 32 keys
+            umma_e4m3(tmem_base + O_COL + (it & 1) * 16, a + 2 * j * (32 * HD >> 4), b + 2 * j * (32 * 16 >> 4), idesc, j != 0);
+            umma_e4m3(tmem_base + O_COL + (it & 1) * 16, a + (2 * j + 1) * (32 * HD >> 4), b + (2 * j + 1) * (32 * 16 >> 4), idesc, true);
+          }
         umma_commit(&o_full[it & 1]);
         umma_commit(&vempty[vs]);
         advance(at);
@@ -347,7 +427,8 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     }
   } else {
     // (no way out of this loop: the four warps meet at barriers; once a wait has run out the others are not waited for)
-    const int quarter = warp & 3, st = tid - 64;
+    pdl_wait();
+    const int quarter = warp & 3, st = tid - (DE_THREADS - DE_SOFT);
     const int r = quarter * 32 + lane;                // key of the tile
     const int dim = HD == 128 ? r : quarter * 16 + lane;         // number of the head (heads of 64: a warp's first 16 lanes)
     const bool has_dim = HD == 128 || lane < 16;
@@ -403,11 +484,13 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       if (lane == 0) mbar_arrive(&q_full[buf]);
     };
     DecPlace at = start;
-    prepare(at, 0);
+    if (n_tiles > 0) prepare(at, 0);
     soft_sync();
-    int seg = 0;
+    int seg = 0, k_first = 0;
     bool fresh = true;
-    float m[GM], l[GM], N[GM], n_t[GM], o[GM];
+    float m[GM], l[GM], N[GM], n_t[GM], o[GM], fs[GM];
+    int g0 = 0, GC = 0, head0 = 0, first_key = 0, last_key = 0;       // of the sequence
+    int key = 0;                                      // this thread's first; a second is 128 behind it
     // the output of tile `it`, whose reference is n_t, into o
     auto gather = [&](int it) {
       wait(&o_full[it & 1], it >> 1);
@@ -424,30 +507,45 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
         float x = fmaf(t[GM + g], 0.0625f, t[g]);
         if (TERMS == 3) x = fmaf(t[(TERMS - 1) * GM + g], 0.00390625f, x);
         const float top = fmaxf(N[g], n_t[g]);
-        o[g] = fmaf(o[g], exp2_whole(N[g] - top), x * exp2_whole(n_t[g] - top));
+        o[g] = fmaf(o[g], exp2_fast(N[g] - top), x * exp2_fast(n_t[g] - top));
         N[g] = top;
       }
     };
     for (int it = 0; it < n_tiles; ++it) {
-      const int g0 = at.head % p.n_gchunks * DE_GM, GC = min(GM, G - g0);
       DecPlace next = at;
       const bool ends = advance(next) || it + 1 == n_tiles;
       if (fresh) {
+        g0 = at.head % p.n_gchunks * DE_GM;
+        GC = min(GM, G - g0);
+        head0 = at.head / p.n_gchunks * G + g0;
+        first_key = begin_s[at.b];
+        last_key = pos_s[at.b];
+        key = (first_key / E8_PAGE + 2 * H * at.k) * E8_PAGE + r;
+        k_first = at.k;
 #pragma unroll
         for (int g = 0; g < GM; ++g) {
           m[g] = N[g] = n_t[g] = -1e30f;
           l[g] = o[g] = 0.f;
+          fs[g] = fs_s[(seg & 1) * DE_GM + g];
         }
       }
       if (ends && it + 1 < n_tiles) prepare(next, (seg + 1) & 1);
+      wait(&sc_full[it % DE_SC], it / DE_SC);
+      int kb[H], vb[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        kb[h] = sc_s[(it % DE_SC * H + h) * 256 + r];
+        vb[h] = sc_s[(it % DE_SC * H + h) * 256 + 128 + r];
+      }
       wait(&s_full[it & 1], it >> 1);
       __syncwarp();
       tc_fence_after_sync();
-      float s[16];
-      tmem_ld_32x16(lane_addr + (it & 1) * 16, s);
-      wait(&sc_full[it % DE_SC], it / DE_SC);
-      __syncwarp();
-      const int kb = sc_s[it % DE_SC * 256 + r], vb = sc_s[it % DE_SC * 256 + 128 + r];
+      float s[H][GM == 4 ? 8 : 16];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        if (GM == 4) tmem_ld_32x8(lane_addr + (it & 1) * 32 + h * 16, s[h]);
+        else tmem_ld_32x16(lane_addr + (it & 1) * 32 + h * 16, s[h]);
+      }
       tmem_ld_wait();
       tc_fence_before_sync();
       __syncwarp();
@@ -455,70 +553,83 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
         mbar_arrive(&s_free[it & 1]);
         mbar_arrive(&sc_empty[it % DE_SC]);
       }
-      const int t = (begin_s[at.b] / E8_PAGE + 2 * at.k) * E8_PAGE + r;
-      const bool seen = t >= begin_s[at.b] && t <= pos_s[at.b];
-      const float kpow = e4m3_scale(kb), bexp = (float)(vb - 127);
-      float* red = red_s + (it & 1) * 4 * 2 * DE_GM;
+      bool seen[H];
+      float bexp[H];
+      float* red = red_s + (it & 1) * 4 * DE_GM;
+      float most[GM];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        seen[h] = key + 128 * h >= first_key && key + 128 * h <= last_key;
+        const float kpow = e4m3_scale(kb[h]);
+        bexp[h] = (float)(vb[h] - 127);
+#pragma unroll
+        for (int g = 0; g < GM; ++g) {
+          const float x = fmaf(s[h][GM + g], 0.0625f, s[h][g]) * (kpow * fs[g]);
+          s[h][g] = seen[h] ? x : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < GM; ++g) most[g] = warp_max_redux(fmaxf(s[0][g] + bexp[0], s[H - 1][g] + bexp[H - 1]));
+      if (lane == 0) {
+#pragma unroll
+        for (int g = 0; g < GM; g += 4)
+          *reinterpret_cast<float4*>(red + quarter * DE_GM + g) = make_float4(most[g], most[g + 1], most[g + 2], most[g + 3]);
+      }
+      // (the sums while the others arrive)
 #pragma unroll
       for (int g = 0; g < GM; ++g) {
-        const float x = fmaf(s[GM + g], 0.0625f, s[g]) * (kpow * fs_s[(seg & 1) * DE_GM + g]);
-        s[g] = seen ? x : -INFINITY;
-        const float a = warp_max_redux(s[g]), b = warp_max_redux(s[g] + bexp);
-        if (lane == 0) {
-          red[quarter * 2 * DE_GM + g] = a;
-          red[quarter * 2 * DE_GM + DE_GM + g] = b;
-        }
+        const float m_new = fmaxf(m[g], fmaxf(s[0][g], s[H - 1][g]));
+        l[g] = fmaf(l[g], exp2_fast(m[g] - m_new), exp2_fast(s[0][g] - m_new) + (H == 2 ? exp2_fast(s[H - 1][g] - m_new) : 0.f));
+        m[g] = m_new;
       }
       soft_sync();
       float n_new[GM];
-      uint32_t packed[4];
-      {
-        float w[GM];
 #pragma unroll
-        for (int g = 0; g < GM; ++g) {
-          const float a = fmaxf(fmaxf(red[g], red[2 * DE_GM + g]), fmaxf(red[4 * DE_GM + g], red[6 * DE_GM + g]));
-          const float b = fmaxf(fmaxf(red[DE_GM + g], red[3 * DE_GM + g]), fmaxf(red[5 * DE_GM + g], red[7 * DE_GM + g]));
-          const float m_new = fmaxf(m[g], ceilf(a));
-          n_new[g] = fmaxf(ceilf(b), -1e30f);
-          l[g] = fmaf(l[g], exp2_whole(m[g] - m_new), exp2_fast(s[g] - m_new));
-          m[g] = m_new;
-          w[g] = exp2_fast(s[g] + (bexp - n_new[g] + 8.f));
-        }
-        // terms of the weights: byte term * GM + g of the key's 16
-        auto term = [&](float f) {
-          uint32_t q4[GM / 4];
+      for (int g = 0; g < GM; g += 4) {
+        float4 x = *reinterpret_cast<const float4*>(red + g);
 #pragma unroll
-          for (int k = 0; k < GM; k += 4) {
-            q4[k / 4] = e4m3_quad(w[k] * f, w[k + 1] * f, w[k + 2] * f, w[k + 3] * f);
-            const float2 ab = e4m3_back(q4[k / 4]), cd = e4m3_back(q4[k / 4] >> 16);
-            const float back = 1.f / f;
-            w[k] = fmaf(-ab.x, back, w[k]);
-            w[k + 1] = fmaf(-ab.y, back, w[k + 1]);
-            w[k + 2] = fmaf(-cd.x, back, w[k + 2]);
-            w[k + 3] = fmaf(-cd.y, back, w[k + 3]);
-          }
-          return GM == 4 ? make_uint2(q4[0], 0u) : make_uint2(q4[0], q4[GM / 4 - 1]);
-        };
-        const uint2 a = term(1.f), b = term(16.f);
-        if (GM == 4) {
-          packed[0] = a.x;
-          packed[1] = b.x;
-          packed[2] = term(256.f).x;
-          packed[3] = 0u;
-        } else {
-          packed[0] = a.x;
-          packed[1] = a.y;
-          packed[2] = b.x;
-          packed[3] = b.y;
+        for (int k = 1; k < 4; ++k) {
+          const float4 y = *reinterpret_cast<const float4*>(red + k * DE_GM + g);
+          x = make_float4(fmaxf(x.x, y.x), fmaxf(x.y, y.y), fmaxf(x.z, y.z), fmaxf(x.w, y.w));
         }
+        n_new[g] = fmaxf(x.x, -1e30f);
+        n_new[g + 1] = fmaxf(x.y, -1e30f);
+        n_new[g + 2] = fmaxf(x.z, -1e30f);
+        n_new[g + 3] = fmaxf(x.w, -1e30f);
       }
-      *reinterpret_cast<uint4*>(p_s + (it & 1) * 2048 + r * 16) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-      // value rows that nobody sees may hold anything: zeros, so that 0 times NaN does not come about
-      if (!seen && (r < E8_PAGE || two_pages(at))) {
-        wait(&vfull[it % VST], it / VST);
-        uint8_t* row = v_s + it % VST * STAGE + r * HD;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) *reinterpret_cast<uint4*>(row + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+      for (int h = 0; h < H; ++h) {
+        uint32_t terms[TERMS][GM / 4];   // byte term * GM + g of the key's 16
+        const float up = bexp[h] + 8.f;
+#pragma unroll
+        for (int g = 0; g < GM; g += 4) {
+          __half2 w01 = __floats2half2_rn(exp2_fast(s[h][g] + up - n_new[g]), exp2_fast(s[h][g + 1] + up - n_new[g + 1]));
+          __half2 w23 = __floats2half2_rn(exp2_fast(s[h][g + 2] + up - n_new[g + 2]), exp2_fast(s[h][g + 3] + up - n_new[g + 3]));
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) {
+            const uint32_t a = e4m3_of_half2(w01), b = e4m3_of_half2(w23);
+            terms[k][g / 4] = a | (b << 16);
+            if (k + 1 < TERMS) {         // what the term leaves over, exact, times 16
+              w01 = __hmul2(__hsub2(w01, half2_of_e4m3(a)), __float2half2_rn(16.f));
+              w23 = __hmul2(__hsub2(w23, half2_of_e4m3(b)), __float2half2_rn(16.f));
+            }
+          }
+        }
+        *reinterpret_cast<uint4*>(p_s + ((it & 1) * H + h) * 2048 + r * 16) =
+            GM == 4 ? make_uint4(terms[0][0], terms[1][0], terms[TERMS - 1][0], 0u)
+                    : make_uint4(terms[0][0], terms[0][GM / 4 - 1], terms[1][0], terms[1][GM / 4 - 1]);
+      }
+      const int n_pages = pages_of(at);
+      if (!seen[0] || !seen[H - 1]) {
+        // value rows that nobody sees may hold anything: zeros, so that 0 times NaN does not come about
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          if (seen[h] || r / E8_PAGE + 2 * h >= n_pages) continue;
+          wait(&vfull[it % VST], it / VST);
+          uint8_t* row = v_s + it % VST * STAGE + (h * 128 + r) * HD;
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) *reinterpret_cast<uint4*>(row + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -527,26 +638,46 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
       for (int g = 0; g < GM; ++g) n_t[g] = n_new[g];
       fresh = ends;
+      key += 128 * H;
       if (ends) {
         gather(it);
         // the sequence's result, or this block's part of it
-        const long long begin = (long long)at.head * P + first[at.b], end = (long long)at.head * P + first[at.b + 1];
-        const bool whole = begin >= lo && end <= hi;
-        const int head0 = at.head / p.n_gchunks * G + g0;
+        const bool whole = k_first == 0 && at.k + 1 == at.nk;
+        // the threads' sums: to the warp's maximum, then half of the heads handed over at every step (a lane ends with one
+        // head's), then the four warps'
+        float mw[GM];
 #pragma unroll
         for (int g = 0; g < GM; ++g) {
-          l[g] = warp_sum(l[g]);
-          if (lane == 0) l_s[quarter * DE_GM + g] = l[g];
+          mw[g] = warp_max_redux(m[g]);
+          l[g] *= exp2_fast(m[g] - mw[g]);
+        }
+#pragma unroll
+        for (int x = 1, n = GM / 2; n > 0; x <<= 1, n >>= 1)
+#pragma unroll
+          for (int g = 0; g < n; ++g) {
+            const float keep = (lane & x) ? l[g + n] : l[g], give = (lane & x) ? l[g] : l[g + n];
+            l[g] = keep + __shfl_xor_sync(0xffffffffu, give, x);
+            if (lane & x) mw[g] = mw[g + n];
+          }
+#pragma unroll
+        for (int x = GM; x < 32; x <<= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
+        if (lane < GM) {
+          int g = 0;
+#pragma unroll
+          for (int x = 1, n = GM / 2; n > 0; x <<= 1, n >>= 1) g += (lane & x) ? n : 0;
+          ml_s[g * 4 + quarter] = make_float2(mw[0], l[0]);
         }
         soft_sync();
-        const size_t part0 = ((size_t)blockIdx.x * 2 + (begin >= lo ? 1 : 0)) * GM;
+        const size_t part0 = ((size_t)blockIdx.x * 2 + (k_first == 0 ? 1 : 0)) * GM;      // (a block shares two at most)
 #pragma unroll
         for (int g = 0; g < GM; ++g) {
           if (g >= GC) continue;
-          float ll = (l_s[g] + l_s[DE_GM + g]) + (l_s[2 * DE_GM + g] + l_s[3 * DE_GM + g]);
+          const float2 w0 = ml_s[g * 4], w1 = ml_s[g * 4 + 1], w2 = ml_s[g * 4 + 2], w3 = ml_s[g * 4 + 3];
+          m[g] = fmaxf(fmaxf(w0.x, w1.x), fmaxf(w2.x, w3.x));
+          float ll = fmaf(w0.y, exp2_fast(w0.x - m[g]), w1.y * exp2_fast(w1.x - m[g])) +
+                     fmaf(w2.y, exp2_fast(w2.x - m[g]), w3.y * exp2_fast(w3.x - m[g]));
           // relative to m (in two steps: the values' powers may be far from the weights')
-          const float half = floorf(0.5f * (N[g] - 8.f - m[g]));
-          const float x = o[g] * exp2_whole(fminf(half, 127.f)) * exp2_whole(fminf(N[g] - 8.f - m[g] - half, 127.f));
+          const float half = exp2_fast(0.5f * (N[g] - 8.f - m[g])), x = o[g] * half * half;
           if (whole) {
             float f = 1.f;
             if (p.sink != nullptr) {
@@ -563,7 +694,8 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
         }
         if (!whole) {
           soft_sync();
-          const int i0 = block_of(begin), parts = block_of(end - 1) - i0 + 1;
+          const long long unit = (long long)at.head * P + first[at.b];
+          const int i0 = block_of(unit), parts = block_of(unit + (at.nk == 1 ? 0 : at.nk)) - i0 + 1;
           if (st == 0) {
             // releases the block's part, which is behind the barrier; acquires those of the blocks before it for the
             // other threads, behind the next one
@@ -575,7 +707,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
           }
           soft_sync();
           if (last) {
-            // a thread per four numbers, or 2, 4, 8 threads that share the parts; four parts in flight each
+            // a thread per four numbers, or 2, 4, 8 threads that share the parts; eight parts in flight each (four where registers are short)
             const int cols = GC * H4;
             int tpc = 1;
             while (tpc < 8 && cols * tpc * 2 <= DE_SOFT) tpc *= 2;
@@ -584,11 +716,11 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
               const int g = min(col, cols - 1) / H4, d = min(col, cols - 1) % H4 * 4;
               float mm = -1e30f, ll = 0.f;
               float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-              for (int k0 = st % tpc; k0 < parts; k0 += 4 * tpc) {
-                float2 ml[4];
-                float4 v[4];
+              for (int k0 = st % tpc; k0 < parts; k0 += JN * tpc) {
+                float2 ml[JN];
+                float4 v[JN];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < JN; ++j) {
                   const int k = k0 + j * tpc;
                   const size_t x = ((size_t)(i0 + min(k, parts - 1)) * 2 + (k == 0 ? 1 : 0)) * GM + g;
                   ml[j] = k < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + x) : make_float2(-1e30f, 0.f);
@@ -596,12 +728,12 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
                 float top = mm;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, ml[j].x);
+                for (int j = 0; j < JN; ++j) top = fmaxf(top, ml[j].x);
                 const float keep = exp2_fast(mm - top);
                 mm = top;
                 ll *= keep; a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < JN; ++j) {
                   const float w = exp2_fast(ml[j].x - top);
                   ll = fmaf(w, ml[j].y, ll);
                   a.x = fmaf(w, v[j].x, a.x); a.y = fmaf(w, v[j].y, a.y);
@@ -651,10 +783,10 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
   }
 }
 
-inline int decode_e8_blocks(int hd) {
+inline int decode_e8_blocks() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms * (hd <= 64 ? de_blocks<64> : de_blocks<128>);
+  return sms * DE_BLOCKS;
 }
 
 template <int HD, int GM>
@@ -665,7 +797,7 @@ int launch_decode_e8(const CUtensorMap& mk, const CUtensorMap& mv, const DecE8& 
     e = cudaFuncSetAttribute((const void*)attention_decode_e4m3_kernel<HD, GM>, cudaFuncAttributePreferredSharedMemoryCarveout,
                              (int)cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return (int)e;
-  launch_kernel(attention_decode_e4m3_kernel<HD, GM>, dim3(decode_e8_blocks(HD)), dim3(DE_THREADS), de_smem<HD>(p.B), stream, mk, mv, p);
+  launch_kernel(attention_decode_e4m3_kernel<HD, GM>, dim3(decode_e8_blocks()), dim3(DE_THREADS), de_smem<HD>(p.B), stream, mk, mv, p);
   return launch_status();
 }
 
@@ -709,7 +841,8 @@ int make_map(CUtensorMap* m, const void* base, long long rows, int hd) {
 // Floats of scratch that a launch needs, whatever the number of sequences.
 DLGO_EXPORT long long dlgo_attention_decode_e4m3_scratch(int Hq, int Hkv, int hd) {
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv) return 0;
-  return (long long)decode_e8_blocks(hd) * 2 * (Hq / Hkv <= 4 ? 4 : DE_GM) * (hd + 2);
+  const int gm = Hq / Hkv <= 4 ? 4 : DE_GM;
+  return (long long)decode_e8_blocks() * 2 * gm * (hd + 2);
 }
 
 // q[B, .] bf16 (row stride ldq, head h at column h * hd), one token per sequence at position token_pos[b] whose key and
@@ -738,7 +871,7 @@ DLGO_EXPORT int dlgo_attention_decode_e4m3(const void* q, int B, int ldq, const 
   p.n_gchunks = (G + DE_GM - 1) / DE_GM;
   p.span = span; p.scale_log2e = scale * 1.4426950408889634f; p.sink = sink;
   p.part_acc = scratch;
-  p.part_ml = scratch + (size_t)decode_e8_blocks(hd) * 2 * gm * hd;
+  p.part_ml = scratch + (size_t)decode_e8_blocks() * 2 * gm * hd;
   for (int b0 = 0; b0 < B; b0 += DE_MAX_B) {       // (one launch as a rule; they run one after another and share the scratch)
     p.B = B - b0 < DE_MAX_B ? B - b0 : DE_MAX_B;
     p.q = (const __nv_bfloat16*)q + (size_t)b0 * ldq;

@@ -1469,39 +1469,51 @@ def e4m3_takes(head_dim: int, page_size: int) -> bool:
 def _check_e4m3(what: str, kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor, vscales: torch.Tensor,
                 page_table: torch.Tensor, num_kv_heads: Optional[int] = None, head_dim: Optional[int] = None) -> None:
     """The shapes of the 8-bit cache's tensors fit one another and the given heads."""
-    if kpages.dim() != 4 or not e4m3_takes(kpages.shape[3], kpages.shape[2]) or kpages.shape != vpages.shape:
-        raise KernelError(f"{what}: keys and values must be [pages, kv heads, 64, 64 or 128], are {tuple(kpages.shape)} and {tuple(vpages.shape)}")
-    if kscales.shape != kpages.shape[:3] or vscales.shape != kpages.shape[:3]:
-        raise KernelError(f"{what}: a scale byte per row: {tuple(kpages.shape[:3])}, not {tuple(kscales.shape)} and {tuple(vscales.shape)}")
-    if page_table.dim() != 2 or page_table.numel() == 0 or kpages.shape[0] == 0:
+    shape = kpages.shape
+    if len(shape) != 4 or shape[2] != E4M3_PAGE or shape[3] not in (64, 128) or shape != vpages.shape:
+        raise KernelError(f"{what}: keys and values must be [pages, kv heads, 64, 64 or 128], are {tuple(shape)} and {tuple(vpages.shape)}")
+    rows = shape[:3]
+    if kscales.shape != rows or vscales.shape != rows:
+        raise KernelError(f"{what}: a scale byte per row: {tuple(rows)}, not {tuple(kscales.shape)} and {tuple(vscales.shape)}")
+    if page_table.dim() != 2 or page_table.numel() == 0 or shape[0] == 0:
         raise KernelError(f"{what}: the page table must be [slots, pages per sequence] and the cache hold a page")
-    if num_kv_heads is not None and (num_kv_heads != kpages.shape[1] or head_dim != kpages.shape[3]):
+    if num_kv_heads is not None and (num_kv_heads != shape[1] or head_dim != shape[3]):
         raise KernelError(f"{what}: the cache's pages do not fit {num_kv_heads} heads of {head_dim}")
 
 
-def _need_e4m3(what: str, here: torch.Tensor, *tensors: tuple) -> None:
-    """Every (name, tensor, type) is contiguous, of that type and on ``here``'s GPU."""
+def _need_e4m3(what: str, device: int, *tensors: tuple) -> None:
+    """Every (name, tensor, type) is contiguous, of that type and on GPU ``device``."""
     for name, t, dt in tensors:
-        _need(t, dt, f"{what}: {name}")
-        if t.device != here.device:
-            raise KernelError(f"{what}: {name} lies on {t.device}, not on {here.device}")
+        if t.dtype is not dt or t.get_device() != device or device < 0 or not t.is_contiguous():
+            _need(t, dt, f"{what}: {name}")
+            raise KernelError(f"{what}: the tensors must live on one GPU (there is no CPU path); {name} lies on {t.device}")
 
 
 def _need_rows(what: str, name: str, t: torch.Tensor, rows: int, cols: int) -> None:
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols or t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] < cols or t.stride(1) != 1:
         raise KernelError(f"{what}: {name} must be 2-D with {rows} rows and {cols} columns next to one another")
 
 
 _E8, _U8, _I32, _F32T = torch.float8_e4m3fn, torch.uint8, torch.int32, torch.float32
 
 
+@functools.lru_cache(maxsize=None)
+def _e4m3_entry(lib: str, name: str, argtypes: str):
+    """The C entry point with its argument types (p: pointer, i: int, f: float), so that plain numbers can be passed."""
+    fn = getattr(_lib(lib), name)
+    fn.argtypes = [{"p": _p, "i": _i, "f": _f}[c] for c in argtypes]
+    return fn
+
+
 def _on_device_of(fn):
     """Run with the first argument's device current, so that the launch goes to that device's current stream."""
     @functools.wraps(fn)
     def call(first: torch.Tensor, *args, **kwargs):
-        if not first.is_cuda or first.device.index == torch._C._cuda_getDevice():
+        index = first.get_device()
+        if index < 0 or index == torch._C._cuda_getDevice():
             return fn(first, *args, **kwargs)
-        with torch.cuda.device(first.device):
+        with torch.cuda.device(index):
             return fn(first, *args, **kwargs)
     return call
 
@@ -1516,8 +1528,8 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, to
     bfloat16.  ``cos`` / ``sin`` [positions, rotary_dim / 2] fp32: the first ``rotary_dim`` numbers of a head are rotated (0: none;
     the tables are then not read), in pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1).  ``write_cache`` False:
     queries only (a layer that reads another's cache).  ``clear`` (fp32): zeros are left where ``qkv`` was read.  A position
-    without a page is not written (:func:`check_device_errors` reports it).  Two tokens of one position in one call: either may
-    be the one that stays."""
+    without a page is not written (:func:`check_device_errors` reports it).  The tokens' positions are distinct within a
+    sequence."""
     what = "rope_append_e4m3"
     if num_heads <= 0 or num_kv_heads <= 0:
         raise KernelError(f"{what}: head counts must be positive")
@@ -1531,20 +1543,21 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, to
         raise KernelError(f"{what}: a position and a sequence per token, and a slot per sequence")
     if not 0 <= rotary_dim <= head_dim or rotary_dim % 2:
         raise KernelError(f"{what}: rotary_dim must be even and no more than {head_dim}")
-    if rotary_dim and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != rotary_dim // 2 or cos.shape[0] == 0):
-        raise KernelError(f"{what}: cos and sin must be [positions, rotary_dim / 2]")
-    if not qkv.is_cuda:
-        raise KernelError(f"{what}: qkv must live on the GPU (there is no CPU path)")
-    _need_e4m3(what, qkv, ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
+    positions = 0
+    if rotary_dim:
+        positions = cos.shape[0]
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != rotary_dim // 2 or positions == 0:
+            raise KernelError(f"{what}: cos and sin must be [positions, rotary_dim / 2]")
+    _need_e4m3(what, qkv.get_device(), ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
                ("page_table", page_table, _I32), ("cos", cos, _F32T), ("sin", sin, _F32T), ("token_pos", token_pos, _I32),
                ("token_seq", token_seq, _I32), ("seq_slot", seq_slot, _I32))
     q = torch.empty((T, num_heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
-    st = _lib("cache_e4m3").dlgo_write_e4m3(
-        _ptr(qkv), _i(code), _i(T), _i(qkv.stride(0) if T > 1 else cols), _ptr(cos), _ptr(sin), _i(cos.shape[0] if rotary_dim else 0),
-        _ptr(token_pos), _ptr(token_seq), _ptr(seq_slot), _ptr(page_table), _i(page_table.shape[0]), _i(page_table.shape[1]), _ptr(kpages),
-        _ptr(vpages), _ptr(kscales), _ptr(vscales), _i(kpages.shape[0]), _ptr(q), _i(num_heads), _i(num_kv_heads), _i(head_dim),
-        _i(rotary_dim), _i(1 if interleaved else 0), _i(1 if write_cache else 0), _i(1 if clear else 0), _stream())
-    _check(st, "rope_append_e4m3", 1 if T > 0 else 0)
+    st = _e4m3_entry("cache_e4m3", "dlgo_write_e4m3", "piiippipppp" + "iipppp" + "ipiiiiiiip")(
+        qkv.data_ptr(), code, T, qkv.stride(0) if T > 1 else cols, cos.data_ptr(), sin.data_ptr(), positions, token_pos.data_ptr(),
+        token_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.shape[0], page_table.shape[1], kpages.data_ptr(),
+        vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(), kpages.shape[0], q.data_ptr(), num_heads, num_kv_heads, head_dim,
+        rotary_dim, interleaved, write_cache, clear, _stream())
+    _check(st, what, 1 if T > 0 else 0)
     return q
 
 
@@ -1558,32 +1571,32 @@ def read_pages_e4m3(kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.T
     _check_e4m3(what, kpages, vpages, kscales, vscales, page_table)
     if pages.dim() != 2 or pages.shape[1] != 3:
         raise KernelError(f"{what}: pages must be [n, 3]: slot, page of its sequence, rows")
-    shape = (pages.shape[0],) + tuple(kpages.shape[1:])
-    for n, t in (("keys", keys), ("values", values)):
+    n, hkv, hd = pages.shape[0], kpages.shape[1], kpages.shape[3]
+    shape = (n, hkv, E4M3_PAGE, hd)
+    for name, t in (("keys", keys), ("values", values)):
         if t is not None and tuple(t.shape) != shape:
-            raise KernelError(f"{what}: {n} must be {shape}, is {tuple(t.shape)}")
+            raise KernelError(f"{what}: {name} must be {shape}, is {tuple(t.shape)}")
     keys = torch.empty(shape, dtype=torch.bfloat16, device=kpages.device) if keys is None else keys
     values = torch.empty(shape, dtype=torch.bfloat16, device=kpages.device) if values is None else values
-    _need_e4m3(what, kpages, ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
+    _need_e4m3(what, kpages.get_device(), ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
                ("page_table", page_table, _I32), ("pages", pages, _I32), ("keys", keys, torch.bfloat16), ("values", values, torch.bfloat16))
-    st = _lib("cache_e4m3").dlgo_read_e4m3(
-        _ptr(kpages), _ptr(vpages), _ptr(kscales), _ptr(vscales), _i(kpages.shape[0]), _ptr(page_table), _i(page_table.shape[0]),
-        _i(page_table.shape[1]), _ptr(pages), _i(pages.shape[0]), _ptr(keys), _ptr(values), _i(kpages.shape[1]), _i(kpages.shape[3]),
-        _stream())
-    _check(st, "read_pages_e4m3", 1 if pages.shape[0] else 0)
+    st = _e4m3_entry("cache_e4m3", "dlgo_read_e4m3", "ppppipiipippiip")(
+        kpages.data_ptr(), vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(), kpages.shape[0], page_table.data_ptr(),
+        page_table.shape[0], page_table.shape[1], pages.data_ptr(), n, keys.data_ptr(), values.data_ptr(), hkv, hd, _stream())
+    _check(st, what, 1 if n else 0)
     return keys, values
 
 
-def attention_decode_e4m3_scratch(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
-    """Floats of scratch of :func:`attention_decode_e4m3`, whatever the number of sequences."""
-    return int(_e4m3_scratch_fn()(_i(num_heads), _i(num_kv_heads), _i(head_dim)))
-
-
-@functools.lru_cache(maxsize=None)
-def _e4m3_scratch_fn():
+@functools.lru_cache(maxsize=256)
+def _e4m3_scratch(device: int, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
     fn = _lib("attention_decode_e4m3").dlgo_attention_decode_e4m3_scratch
     fn.restype = ctypes.c_longlong
-    return fn
+    return int(fn(_i(num_heads), _i(num_kv_heads), _i(head_dim)))
+
+
+def attention_decode_e4m3_scratch(num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Floats of scratch of :func:`attention_decode_e4m3` on the current device, whatever the number of sequences."""
+    return _e4m3_scratch(torch._C._cuda_getDevice(), num_heads, num_kv_heads, head_dim)
 
 
 @_on_device_of
@@ -1606,28 +1619,32 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
     _need_rows(what, "q", q, B, cols)
     if out is None:
         out = torch.empty((B, cols), dtype=torch.bfloat16, device=q.device)
-    _need_rows(what, "out", out, B, cols)
+    else:
+        _need_rows(what, "out", out, B, cols)
     if seq_slot.numel() < B or token_pos.numel() < B:
         raise KernelError(f"{what}: a slot and a position per sequence")
     if sink is not None and sink.numel() != num_heads:
-        raise KernelError("a sink is one number per query head")
-    if not q.is_cuda or not out.device == q.device or q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise KernelError(f"{what}: a sink is one number per query head")
+    device = q.get_device()
+    if device < 0 or out.get_device() != device or q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise KernelError(f"{what}: q and out must be bfloat16 and live on one GPU (there is no CPU path)")
-    floats = attention_decode_e4m3_scratch(num_heads, num_kv_heads, head_dim)
+    floats = _e4m3_scratch(device, num_heads, num_kv_heads, head_dim)
     n_tickets = B * num_kv_heads * ((num_heads // num_kv_heads + 7) // 8)
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if scratch is None else scratch
     tickets = torch.zeros(n_tickets, dtype=torch.int32, device=q.device) if tickets is None else tickets
     if scratch.numel() < floats or tickets.numel() < n_tickets:
         raise KernelError(f"{what}: {floats} floats of scratch and {n_tickets} tickets are needed")
-    _need_e4m3(what, q, ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
+    _need_e4m3(what, device, ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
                ("page_table", page_table, _I32), ("seq_slot", seq_slot, _I32), ("token_pos", token_pos, _I32),
-               ("scratch", scratch, _F32T), ("tickets", tickets, _I32), *((("sink", sink, _F32T),) if sink is not None else ()))
-    st = _lib("attention_decode_e4m3").dlgo_attention_decode_e4m3(
-        _ptr(q), _i(B), _i(q.stride(0) if B > 1 else cols), _ptr(kpages), _ptr(vpages), _ptr(kscales), _ptr(vscales), _i(kpages.shape[0]),
-        _ptr(page_table), _i(page_table.shape[0]), _i(page_table.shape[1]), _ptr(seq_slot), _ptr(token_pos), _ptr(out),
-        _i(out.stride(0) if B > 1 else cols), _i(num_heads), _i(num_kv_heads), _i(head_dim), _i(window), _f(scale), _ptr(sink), _ptr(scratch),
-        _ptr(tickets), _stream())
-    _check(st, "attention_decode_e4m3", 1 if B > 0 else 0)
+               ("scratch", scratch, _F32T), ("tickets", tickets, _I32))
+    if sink is not None:
+        _need_e4m3(what, device, ("sink", sink, _F32T))
+    st = _e4m3_entry("attention_decode_e4m3", "dlgo_attention_decode_e4m3", "piippppipiipppiiiiifpppp")(
+        q.data_ptr(), B, q.stride(0) if B > 1 else cols, kpages.data_ptr(), vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(),
+        kpages.shape[0], page_table.data_ptr(), page_table.shape[0], page_table.shape[1], seq_slot.data_ptr(), token_pos.data_ptr(),
+        out.data_ptr(), out.stride(0) if B > 1 else cols, num_heads, num_kv_heads, head_dim, window, scale,
+        0 if sink is None else sink.data_ptr(), scratch.data_ptr(), tickets.data_ptr(), _stream())
+    _check(st, what, 1 if B > 0 else 0)
     return out
 
 
