@@ -47,21 +47,30 @@ __device__ __forceinline__ long long e8_row(const WriteE8& p, int t, int& pos, b
   return (long long)page * p.Hkv * E8_PAGE + pos % E8_PAGE;
 }
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&o)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&o)[8]) {
-  const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
-  o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&o)[8]) {
-  const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p));
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    o[2 * i] = f.x;
-    o[2 * i + 1] = f.y;
+// eight numbers as they lie in memory, and as fp32
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldcg(reinterpret_cast<const float4*>(p));
+    b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
   }
-}
+  __device__ __forceinline__ void numbers(float (&o)[8]) const {
+    o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
+  }
+};
+template <> struct Eight<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = __ldcg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void numbers(float (&o)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
 __device__ __forceinline__ void clear8(float* p) {
   reinterpret_cast<float4*>(p)[0] = make_float4(0.f, 0.f, 0.f, 0.f);
   reinterpret_cast<float4*>(p)[1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -98,21 +107,27 @@ __global__ void __launch_bounds__(WE_WARPS * 32) write_e4m3_kernel(WriteE8 p, in
     }
   }
   pdl_wait();
-  T* row = (T*)p.qkv + (size_t)t * p.ld;
-  for (int h0 = part * HEADS; h0 < n_heads; h0 += per_token * HEADS) {
+  T* row = (T*)p.qkv + (size_t)t * p.ld + i;
+  const int stride = per_token * HEADS;
+  Eight<T> ahead[2] = {};
+  const int head_first = part * HEADS + lane / LANES;
+  if (head_first < n_heads) {
+    ahead[0].load(row + (size_t)head_first * HD);
+    ahead[1].load(row + (size_t)head_first * HD + HD / 2);
+  }
+  for (int h0 = part * HEADS; h0 < n_heads; h0 += stride) {
     const int head = h0 + lane / LANES;
     const bool here = head < n_heads;
     float lo[8], hi[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) lo[k] = hi[k] = 0.f;
-    T* src = row + (size_t)head * HD + i;
-    if (here) {
-      load8<T>(src, lo);
-      load8<T>(src + HD / 2, hi);
-      if (p.clear) {
-        clear8(src);
-        clear8(src + HD / 2);
-      }
+    ahead[0].numbers(lo);
+    ahead[1].numbers(hi);
+    if (head + stride < n_heads) {                 // the next round's, while this one is worked on
+      ahead[0].load(row + (size_t)(head + stride) * HD);
+      ahead[1].load(row + (size_t)(head + stride) * HD + HD / 2);
+    }
+    if (p.clear && here) {
+      clear8(row + (size_t)head * HD);
+      clear8(row + (size_t)head * HD + HD / 2);
     }
     if (head < p.Hq + p.Hkv) {
 #pragma unroll
