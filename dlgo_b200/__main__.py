@@ -43,6 +43,7 @@ def _add_generation_options(p: argparse.ArgumentParser) -> None:
     p.add_argument("--profile", action="store_true",
                    help="time every kernel (CUDA events, no CUDA graphs) and print the totals; also DLGO_PROFILE=1")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    p.add_argument("--cache-dtype", default=None, choices=["e4m3"], help="keep keys and values in 8 bits (default: as --dtype)")
     p.add_argument("--device", default="cuda:0")
     p.add_argument("--max-batch", type=int, default=64)
 
@@ -62,7 +63,8 @@ def _cmd_generate(a: argparse.Namespace) -> int:
         return 2
     import os
     profile = a.profile or os.environ.get("DLGO_PROFILE", "") not in ("", "0")
-    llm = load_llm(a.model, a.ctx, dtype=a.dtype, device=a.device, max_batch=a.max_batch, cuda_graphs=not profile)
+    llm = load_llm(a.model, a.ctx, dtype=a.dtype, device=a.device, max_batch=a.max_batch, cuda_graphs=not profile,
+                   cache_dtype=a.cache_dtype)
     print(f"Model: {llm.model_info()}", file=sys.stderr)
     if profile:
         from .csrc import kernels

@@ -183,15 +183,17 @@ class LLM:
 
 
 def load_llm(model_path: str, max_seq_len: int = 0, *, dtype: str = "bfloat16", device: str = "cuda:0",
-             max_tokens: Optional[int] = None, max_batch: int = 64, cuda_graphs: bool = True) -> LLM:
+             max_tokens: Optional[int] = None, max_batch: int = 64, cuda_graphs: bool = True,
+             cache_dtype: Optional[str] = None) -> LLM:
     """Load a model folder (config.json + model.safetensors) and return a ready LLM.
 
     ``max_seq_len`` is the longest sequence (0 = the model's context), as in the
     reference's ``LoadLLM(path, maxSeqLen)`` (dlgo.go:37-48).  ``max_tokens`` sizes the
     cache: positions that live sequences may hold together (default: ``max_batch``
-    sequences of ``max_seq_len``, within half of the device's free memory).
+    sequences of ``max_seq_len``, within half of the device's free memory).  ``cache_dtype="e4m3"`` keeps
+    keys and values in 8 bits: half the bytes to hold and to read for every token.
     """
     engine = Engine(model_path, dtype=dtype, device=device, max_tokens=max_tokens,
                     max_seq_len=max_seq_len if max_seq_len > 0 else None, cuda_graphs=cuda_graphs,
-                    default_batch=max_batch)
+                    default_batch=max_batch, cache_dtype=cache_dtype)
     return LLM(engine, max_batch=max_batch)

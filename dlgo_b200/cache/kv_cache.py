@@ -2,7 +2,7 @@
 
 Per group of run entries with equal needs, ONE allocation
 ``[entries, planes (keys, values; or one for both), pages, kv_heads, page_size, head_dim]`` in the
-run's precision and one page table ``[slots, pages per sequence]`` (int32, -1
+run's precision (or in 8 bits: e4m3 numbers, beside one scale byte per row of a head) and one page table ``[slots, pages per sequence]`` (int32, -1
 where no page is held).  The layout keeps one kv head's 64 positions of a page
 contiguous, which is what the attention kernel streams.
 
@@ -35,6 +35,8 @@ class CacheView:
     page_table: torch.Tensor    # [slots, pages per sequence] int32
     page_size: int
     writes: bool                # False when the entry reads another entry's cache
+    key_scales: Optional[torch.Tensor] = None      # [pages, kv_heads, page_size] uint8 where keys and values are e4m3 numbers
+    value_scales: Optional[torch.Tensor] = None
 
 
 class StateArea:
@@ -71,12 +73,13 @@ class KVCache:
     ``entry_needs[i]`` is what run entry ``i`` keeps (``None``: nothing, or it
     borrows: then ``borrows[i]`` names the lender).  ``max_tokens`` is the number
     of positions live sequences may hold in total, each sequence's count rounded
-    up to a whole page.
+    up to a whole page.  ``e4m3``: keys and values as 8-bit rows with a power of two each (kernels.rope_append_e4m3 has the
+    definition) instead of ``dtype``.
     """
 
     def __init__(self, entry_needs: Sequence[Optional[CacheNeed]], borrows: Sequence[Optional[int]],
                  state_needs: Dict[int, StateNeed], max_tokens: int, max_seq_len: int, dtype: torch.dtype,
-                 device: torch.device, page_size: int = PAGE_SIZE, n_slots: Optional[int] = None):
+                 device: torch.device, page_size: int = PAGE_SIZE, n_slots: Optional[int] = None, e4m3: bool = False):
         self.page_size = page_size
         n_pages = max(1, (max_tokens + page_size - 1) // page_size)
         self.n_pages = n_pages
@@ -98,13 +101,17 @@ class KVCache:
         self.book = CacheBook([(names[k], k[3]) for k in keyed], n_pages, page_size, self.n_slots, self.max_seq_len)
         self._no_window = all(k[3] is None for k in keyed)
         self.storage: Dict[str, torch.Tensor] = {}
+        self.scales: Dict[str, torch.Tensor] = {}      # (8-bit storage: a scale byte per row of a head)
+        self.e4m3 = e4m3
         self.page_tables: Dict[str, torch.Tensor] = {}
         self._entry_place: Dict[int, Tuple[str, int]] = {}
         for key, entries in keyed.items():
             name = names[key]
             _, hkv, hd, _, planes = key
-            self.storage[name] = torch.empty((len(entries), planes, n_pages, hkv, page_size, hd), dtype=dtype,
-                                             device=device)
+            rows = (len(entries), planes, n_pages, hkv, page_size)
+            self.storage[name] = torch.empty(rows + (hd,), dtype=torch.uint8 if e4m3 else dtype, device=device)
+            if e4m3:
+                self.scales[name] = torch.empty(rows, dtype=torch.uint8, device=device)
             self.page_tables[name] = torch.full((self.n_slots, self.book.max_pages_per_seq), -1, dtype=torch.int32,
                                                 device=device)
             for j, e in enumerate(entries):
@@ -123,11 +130,15 @@ class KVCache:
             return None
         name, j = place
         st = self.storage[name]
+        if self.e4m3:
+            sc = self.scales[name]
+            st = st.view(torch.float8_e4m3fn)
+            return CacheView(st[j, 0], st[j, 1], self.page_tables[name], self.page_size, src == entry, sc[j, 0], sc[j, 1])
         # (one plane: the rows serve as keys and as values)
         return CacheView(st[j, 0], st[j, st.shape[1] - 1], self.page_tables[name], self.page_size, writes=src == entry)
 
     def bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self.storage.values())
+        return sum(t.numel() * t.element_size() for d in (self.storage, self.scales) for t in d.values())
 
     # ------------------------------------------------------------------ slots
     def take_slot(self) -> int:
@@ -142,7 +153,7 @@ class KVCache:
         if self.poison_freed:
             for g, pages in released.items():
                 if pages:
-                    self.storage[g][:, :, torch.tensor(pages, device=self.device)] = float("nan")
+                    self.storage[g][:, :, torch.tensor(pages, device=self.device)] = 0x7F if self.e4m3 else float("nan")
 
     def length(self, slot: int) -> int:
         return self.book.length(slot)
@@ -180,7 +191,9 @@ class KVCache:
         """Fill every page with ``value`` (tests: nothing unwritten may reach a result)."""
         self.poison_freed = True
         for st in self.storage.values():
-            st.fill_(value)
+            st.fill_(0x7F if self.e4m3 else value)      # (an e4m3 NaN)
+        for sc in self.scales.values():
+            sc.fill_(255)
 
 
 __all__ = ["CacheError", "CacheView", "KVCache", "PAGE_SIZE", "StateArea"]

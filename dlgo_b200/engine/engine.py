@@ -24,26 +24,46 @@ from ..config.registry import load_config
 from ..weights.loader import DictSource, WeightSource
 from .graphs import decode_with_graph, greedy_with_graph, sampled_with_graph
 from .model import CausalLM
-from .runtime import Runtime, build_context
+from .runtime import Runtime, build_context, parse_dtype
 
 
 class StepError(ValueError):
     """A step the engine refuses (bad token id, unknown slot, sequence too long)."""
 
 
+def _e4m3_cache(cache_dtype: Optional[str], dtype: Any) -> bool:
+    """Whether the cache keeps 8-bit rows: ``cache_dtype`` is ``None`` or the run's own type, or ``"e4m3"``."""
+    if cache_dtype is None:
+        return False
+    if str(cache_dtype).lower() in ("e4m3", "float8_e4m3fn", "torch.float8_e4m3fn"):
+        if parse_dtype(dtype) != torch.bfloat16:
+            raise ValueError("cache_dtype 'e4m3' goes with bfloat16 runs (float32 keeps everything in 32 bits)")
+        return True
+    try:
+        same = parse_dtype(cache_dtype) == parse_dtype(dtype)
+    except ValueError:
+        same = False
+    if not same:
+        raise ValueError(f"cache_dtype must be 'e4m3' or the run's own type, not {cache_dtype!r}")
+    return False
+
+
 class Engine:
     def __init__(self, model_dir: Optional[str] = None, dtype="bfloat16", device="cuda:0",
                  max_tokens: Optional[int] = None, max_seq_len: Optional[int] = None, cuda_graphs: bool = True,
                  default_batch: int = 1, spec: Any = None, tensors: Optional[Dict[str, torch.Tensor]] = None,
-                 max_slots: Optional[int] = None):
+                 max_slots: Optional[int] = None, cache_dtype: Optional[str] = None):
         """``max_tokens``: positions live sequences may hold in total (each sequence's count
         rounded up to a multiple of 64); it sizes the cache.  ``max_seq_len``: longest single
         sequence, clamped to the model's context like the reference's ``maxSeqLen``
         (models/llm/generate.go:56-58).  ``max_slots``: sequences that may be live at once (default:
         one per page of the cache, but no more than keep a group's page table within 64 MB).
+        ``cache_dtype``: ``"e4m3"`` keeps keys and values in 8 bits, a power of two per row of a head beside them: half the bytes
+        per position, for bfloat16 runs whose layers are grouped-query attention with heads of 64 or 128 (default: ``dtype``).
 
         A model comes from ``model_dir`` (config.json chooses the architecture), or from an
         :class:`ArchitectureSpec` and its tensors given in memory (``spec``, ``tensors``)."""
+        e4m3 = _e4m3_cache(cache_dtype, dtype)
         self.runtime = Runtime(device, dtype)
         if spec is None:
             if model_dir is None:
@@ -54,6 +74,8 @@ class Engine:
             self.config = None
             self.spec = spec
         self.model = CausalLM(self.spec)
+        if e4m3:
+            self._check_e4m3_cache()
         with torch.cuda.device(self.runtime.device):
             if tensors is not None:
                 source = DictSource(tensors, self.runtime.device)
@@ -68,8 +90,9 @@ class Engine:
         needs, borrows, states = self.model.cache_needs()
         if max_tokens is None or max_tokens <= 0:
             # room for `default_batch` sequences of full length, within half of the free memory
-            per_position = sum(n.planes * n.num_kv_heads * n.head_dim for n, b in zip(needs, borrows)
-                               if n is not None and b is None) * (2 if self.runtime.dtype == torch.bfloat16 else 4)
+            size = 2 if self.runtime.dtype == torch.bfloat16 else 4
+            per_position = sum(n.planes * n.num_kv_heads * (n.head_dim + 1 if e4m3 else n.head_dim * size)
+                               for n, b in zip(needs, borrows) if n is not None and b is None)
             free, _ = torch.cuda.mem_get_info(self.runtime.device)
             fits = max(PAGE_SIZE, int(free * 0.5) // max(per_position, 1))
             max_tokens = max(min(max_seq_len * max(default_batch, 1), fits), min(max_seq_len, fits))
@@ -80,13 +103,28 @@ class Engine:
             row_bytes = 4 * ((min(max_seq_len, n_pages * PAGE_SIZE) + PAGE_SIZE - 1) // PAGE_SIZE)
             max_slots = min(n_pages, max(default_batch, 256, (64 << 20) // row_bytes))
         self.cache = KVCache(needs, borrows, states, max_tokens, max_seq_len, self.runtime.dtype, self.runtime.device,
-                             PAGE_SIZE, n_slots=max_slots)
+                             PAGE_SIZE, n_slots=max_slots, e4m3=e4m3)
         self.max_seq_len = self.cache.max_seq_len
         self.vocab_size = self.spec.vocab_size
         self.cuda_graphs = cuda_graphs
         self._graphs: "OrderedDict[tuple, object]" = OrderedDict()    # (batch size, reach) -> captured step
         self._graph_pool = None
         self.launches_last_step = 0
+
+    def _check_e4m3_cache(self) -> None:
+        """Every layer that keeps keys and values, or reads another's, must be able to keep them in 8 bits."""
+        kept = 0
+        for i, entry in enumerate(self.model.order):
+            mixer = self.model.blocks[entry.layer].mixer
+            need = mixer.cache_need() if mixer is not None else None
+            if need is None:
+                continue
+            if not mixer.takes_e4m3_cache() or need.planes != 2:
+                raise ValueError(f"cache_dtype 'e4m3' is for grouped-query attention with heads of 64 or 128; run entry {i} "
+                                 f"({type(mixer).__name__}, heads of {need.head_dim}) keeps its cache in the run's precision")
+            kept += 1
+        if not kept:
+            raise ValueError("cache_dtype 'e4m3': no layer of this model keeps keys and values")
 
     def _note_stand_ins(self) -> None:
         """One line on stderr when a bfloat16 model's sizes land on the slower stand-in kernels (never a wrong

@@ -68,7 +68,7 @@ class FusedRun:
     def takes(self, ctx: Any, cache: Any) -> bool:
         d, hq, hkv, hd, f = self.sig[:5]
         view = cache.view(self.first)
-        return (ctx.decode and ctx.n_tokens <= MAX_TOKENS and view is not None and
+        return (ctx.decode and ctx.n_tokens <= MAX_TOKENS and view is not None and view.keys.dtype == torch.bfloat16 and
                 K.decode_layers_takes(ctx.n_tokens, d, hq, hkv, hd, f, view.page_size))
 
     def _descriptors(self, model: Any, cache: Any, device: torch.device) -> torch.Tensor:

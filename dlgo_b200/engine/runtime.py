@@ -88,6 +88,7 @@ class StepContext:
     sublayer_input_f32: Optional[torch.Tensor] = None   # the fp32 stream a sublayer reads, where its block offers it
     normed_ahead: Optional[tuple] = None     # (residual stream, norm, its rows normed by that norm): made by a block's last launch for its successor
     _tiles: Dict[Tuple[int, bool], Tuple[torch.Tensor, int, int]] = field(default_factory=dict)
+    _pages: Dict[int, Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = field(default_factory=dict)
     _scratch: Dict[str, torch.Tensor] = field(default_factory=dict)
 
     def tiles(self, tokens_per_tile: int, heaviest_first: bool = False) -> Tuple[torch.Tensor, int, int]:
@@ -114,6 +115,29 @@ class StepContext:
         t = torch.tensor(rows, dtype=torch.int32).to(self.runtime.device, non_blocking=True)
         self._tiles[(tokens_per_tile, heaviest_first)] = (t, len(rows), biggest)
         return self._tiles[(tokens_per_tile, heaviest_first)]
+
+    def pages_in_sight(self, span: int, page_size: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The pages that the step's queries see, for a copy of them one after another (outside a capture): (device tensor
+        [n, 3] of (slot, page of its sequence, positions it holds after this step), a page table [sequences, pages] that maps
+        a sequence's page to its number in that list, -1 where no query sees it, and the sequences' rows of that table).
+        ``span``: what a query sees, as the attention kernels take it."""
+        hit = self._pages.get(span)
+        if hit is not None:
+            return hit
+        rows: List[Tuple[int, int, int]] = []
+        places: List[List[int]] = []
+        for slot, start, n in zip(self.seq_slots_host, self.seq_start_host, self.seq_ntok_host):
+            first = max(0, start - span + 1) if span > 0 else (start - start % -span if span < 0 else 0)
+            lo, hi = first // page_size, (start + n - 1) // page_size
+            places.append([-1] * lo + list(range(len(rows), len(rows) + hi + 1 - lo)))
+            rows.extend((slot, p, min(page_size, start + n - p * page_size)) for p in range(lo, hi + 1))
+        width = max(len(p) for p in places)
+        dev = self.runtime.device
+        table = torch.tensor([p + [-1] * (width - len(p)) for p in places], dtype=torch.int32)
+        hit = (torch.tensor(rows, dtype=torch.int32).to(dev, non_blocking=True), table.to(dev, non_blocking=True),
+               torch.arange(len(places), dtype=torch.int32).to(dev, non_blocking=True))
+        self._pages[span] = hit
+        return hit
 
     def scratch(self, name: str, numel: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """A scratch buffer that lives for the step (shared by the layers, which run one after another)."""

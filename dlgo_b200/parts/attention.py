@@ -108,6 +108,10 @@ class GQAAttention(Mixer):
             return self.window
         return -self.chunk if self.chunk else 0
 
+    def takes_e4m3_cache(self) -> bool:
+        # (a subclass with a forward of its own appends to the cache itself)
+        return type(self).forward is GQAAttention.forward and K.e4m3_takes(self.head_dim, K.E4M3_PAGE)
+
     # -------------------------------------------------------------------- forward
     def _decode_slices(self, T: int, pages: int, sms: int) -> tuple:
         """(page slices per sequence of the decode kernels, how many would fit): slices so that every SM has several
@@ -230,6 +234,9 @@ class GQAAttention(Mixer):
             rot, inter = 0, False
         act = self.wqkv.weight.dtype
         n_cols = self.q_dim + 2 * self.kv_dim
+        if cache.key_scales is not None:
+            self._forward_e4m3(x, residual, ctx, cache, cos, sin, rot, inter)
+            return
         # bfloat16, common head sizes, one token per sequence: scores and weighted sum on the tensor cores
         decode_kernel, mma, n_splits, scratch, counters, pages = self._decode_plan(ctx, cache, act)
         out = torch.empty((T, self.q_dim), dtype=act, device=x.device)
@@ -272,6 +279,39 @@ class GQAAttention(Mixer):
                           qkv_parts, False)
         if not rotated:
             self._attend(qkv, ctx, cache, out, decode_kernel, mma, n_splits, scratch, counters, pages)
+        self._project_out(out, residual, ctx)
+
+
+    def _forward_e4m3(self, x: torch.Tensor, residual: torch.Tensor, ctx: Any, cache: Any, cos: torch.Tensor,
+                      sin: torch.Tensor, rot: int, inter: bool) -> None:
+        """The same over the 8-bit cache: the projection rotated and its keys and values stored by one kernel; single tokens
+        attend the rows as they are stored, prompts their pages read back as bfloat16 (each is then read by many tokens)."""
+        T, n_cols = ctx.n_tokens, self.q_dim + 2 * self.kv_dim
+        hq, hkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
+        rows = (cache.keys, cache.values, cache.key_scales, cache.value_scales, cache.page_table)
+        clear = bool(_QKV_SUM and self.wqkv.sums_slices_at_memory(T))
+        if clear:
+            # few tokens: the projection's K-slices add themselves into one fp32 sum that is zero between steps
+            proj = ctx.zeros(f"qkv_sum{n_cols}", T * n_cols, torch.float32)[:T * n_cols].view(T, n_cols)
+            self.wqkv(x, ADD_F32, proj)
+        else:
+            proj = self.wqkv(x, STORE_F32 if ctx.decode else STORE)
+        q = K.rope_append_e4m3(proj, cos, sin, ctx.token_pos, ctx.token_seq, ctx.seq_slot, *rows, hq, hkv, hd, rot, inter,
+                               cache.writes, clear)
+        out = torch.empty((T, self.q_dim), dtype=torch.bfloat16, device=x.device)
+        if ctx.decode:
+            K.attention_decode_e4m3(q, *rows, ctx.seq_slot, ctx.token_pos, hq, hkv, hd, self.scale, self.span(), self.sink, out,
+                                    ctx.scratch("attention_e4m3", K.attention_decode_e4m3_scratch(hq, hkv, hd)),
+                                    ctx.zeros("attention_e4m3_tickets", T * hkv * ((hq // hkv + 7) // 8)))
+        else:
+            pages, table, at = ctx.pages_in_sight(self.span(), cache.page_size)
+            shape = (pages.shape[0], hkv, cache.page_size, hd)
+            n = pages.shape[0] * hkv * cache.page_size * hd
+            keys, values = (ctx.scratch(f"attention_e4m3_{name}", n, torch.bfloat16)[:n].view(shape) for name in ("keys", "values"))
+            K.read_pages_e4m3(*rows, pages, keys, values)
+            tiles, _, _ = ctx.tiles(K.PREFILL_TC_TILE, heaviest_first=True)
+            K.attention_prefill_tc(q, q.stride(0), T, keys, values, table, tiles, at, ctx.token_pos, out, hq, hkv, hd, self.scale,
+                                   self.span(), sink=self.sink, split=self.split_weights)
         self._project_out(out, residual, ctx)
 
 

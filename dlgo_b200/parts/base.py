@@ -107,6 +107,11 @@ class Mixer(Part):
     def state_need(self) -> Optional[StateNeed]:
         return None
 
+    def takes_e4m3_cache(self) -> bool:
+        """Whether this mixer can keep and read its keys and values as 8-bit rows with a scale each (the cache's view then
+        has ``key_scales`` and ``value_scales``)."""
+        return False
+
     def forward(self, x: torch.Tensor, residual: torch.Tensor, ctx: "Any", cache: "Any",
                 state: Optional[torch.Tensor], positions: Mapping[str, PositionEncoding]) -> None:
         raise NotImplementedError

@@ -83,3 +83,25 @@ def test_operators_name_what_does_not_fit():
     for more, word in ((dict(pages=torch.zeros(1, 2, dtype=torch.int32)), "slot, page"), (dict(keys=torch.zeros(2, 2, 64, 64)), "must be")):
         with pytest.raises(K.KernelError, match=word):
             read(**more)
+
+
+def test_pages_in_sight_of_a_step():
+    """The list of pages that a prompt step copies, and the table that finds them in the copy."""
+    from dlgo_b200.engine.runtime import StepContext
+
+    class Runtime:
+        device = torch.device("cpu")
+
+    def ctx():
+        return StepContext(runtime=Runtime(), n_tokens=0, n_seqs=3, token_ids=None, token_pos=None, token_seq=None, seq_slot=None,
+                           seq_slots_host=[7, 2, 5], seq_start_host=[0, 130, 63], seq_ntok_host=[3, 65, 1], decode=False, max_len=195)
+
+    pages, table, at = ctx().pages_in_sight(0, 64)
+    assert pages.tolist() == [[7, 0, 3], [2, 0, 64], [2, 1, 64], [2, 2, 64], [2, 3, 3], [5, 0, 64]]
+    assert table.tolist() == [[0, -1, -1, -1], [1, 2, 3, 4], [5, -1, -1, -1]] and at.tolist() == [0, 1, 2]
+    pages, table, _ = ctx().pages_in_sight(3, 64)           # a window of 3: the first query at 130 sees 128 on
+    assert pages.tolist() == [[7, 0, 3], [2, 2, 64], [2, 3, 3], [5, 0, 64]] and table.tolist() == [[0, -1, -1, -1], [-1, -1, 1, 2], [3, -1, -1, -1]]
+    pages, table, _ = ctx().pages_in_sight(4, 64)           # 127 on: a page more
+    assert pages.tolist()[1] == [2, 1, 64] and table.tolist()[1] == [-1, 1, 2, 3]
+    pages, table, _ = ctx().pages_in_sight(-100, 64)        # chunks of 100: from position 100 on
+    assert pages.tolist() == [[7, 0, 3], [2, 1, 64], [2, 2, 64], [2, 3, 3], [5, 0, 64]]
