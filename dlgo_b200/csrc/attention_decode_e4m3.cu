@@ -77,8 +77,8 @@ struct DecE8 {
   int ldo, B, Hq, Hkv, n_gchunks, span;
   float scale_log2e;
   const float* sink;       // [Hq] or null: exp(sink) joins the denominator
-  float* part_acc;         // [blocks][2][GM][HD]
-  float* part_ml;          // [blocks][2][GM][2]
+  float* part_acc;         // [blocks][2][GM][HD]  O relative to m
+  float* part_ml;          // [blocks][2][GM][2]  m and l
   int* tickets;            // [B][heads], zero between launches
 };
 
@@ -162,7 +162,7 @@ template <int HD> constexpr int de_off_sc = de_off_p<HD> + 2 * de_halves<HD> * 2
 template <int HD> constexpr int de_off_bars = de_off_sc<HD> + DE_SC * de_halves<HD> * 256;
 template <int HD> constexpr int de_off_red = de_off_bars<HD> + DE_BARS * 8;             // [2][4][GM] floats
 template <int HD> constexpr int de_off_misc = de_off_red<HD> + 2 * 4 * DE_GM * 4;    // row scales [2][GM], maxima and sums [GM][4], words
-template <int HD> constexpr int de_off_seq = de_off_misc<HD> + 10 * DE_GM * 4 + 64;
+template <int HD> constexpr int de_off_seq = de_off_misc<HD> + 10 * DE_GM * 4 + 128;
 template <int HD> constexpr size_t de_smem(int B) { return de_off_seq<HD> + (size_t)(4 * B + 1) * 4; }
 
 template <int HD, int GM>
@@ -171,7 +171,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
   constexpr int TERMS = GM <= 4 ? 3 : 2;
   constexpr int H = de_halves<HD>, KST = DE_KST, VST = DE_VST, STAGE = H * 128 * HD, PAGE_BYTES = E8_PAGE * HD;
   constexpr uint32_t TMEM_COLS = 128, O_COL = 64;     // scores of two tiles in columns 0 to 63, outputs in 64 and 80
-  constexpr int H4 = HD / 4, JN = GM <= 4 ? 8 : 4;
+  constexpr int H4 = HD / 4, JN = 6;
   // the swizzled tiles want 1024-byte alignment (checked: a misaligned start ends the kernel with the error word set)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -201,9 +201,10 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
   float* fs_s = (float*)(smem + de_off_misc<HD>);     // [2][DE_GM] row scales
   float2* ml_s = (float2*)(fs_s + 2 * DE_GM);         // [DE_GM][4 warps] maximum and sum
   int* sums = (int*)(ml_s + 4 * DE_GM);               // [8]
-  int& last = sums[8];
-  uint32_t* tmem_slot = (uint32_t*)(sums + 9);
-  volatile int* abort_flag = sums + 10;
+  uint32_t* tmem_slot = (uint32_t*)(sums + 8);
+  volatile int* abort_flag = sums + 9;
+  int* last_s = sums + 10;                            // [2] this block has a shared sequence's last ticket
+  int* shared_s = sums + 16;                          // [2][4] head, sequence, first block, parts of the sequences it shares
   int* first = (int*)(smem + de_off_seq<HD>);         // [B + 1] first tile of each sequence
   const int B = p.B, G = p.Hq / p.Hkv, heads = p.Hkv * p.n_gchunks;
   int* pos_s = first + B + 1;                         // [B] last visible position
@@ -437,18 +438,36 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     auto wait = [&](uint64_t* bar, int parity) {
       if (ok) ok = mbar_wait(bar, parity & 1, abort_flag);
     };
-    // the queries of a sequence and kv head as two e4m3 terms (rows g and GM + g of the operand), and what the scores are
+    // the queries of a sequence and kv head, fetched when the sequence before begins, as two e4m3 terms (rows g and GM + g of the operand), and what the scores are
     // scaled by; 16 threads a head
-    auto prepare = [&](const DecPlace& x, int buf) {
-      const int g0 = x.head % p.n_gchunks * DE_GM, GC = min(GM, G - g0), head0 = x.head / p.n_gchunks * G + g0;
+    // what a head's weighted sum, relative to m, is multiplied with: 1 / l, the sink's share in l
+    auto finish = [&](int head, float mm, float ll) {
+      float f = 1.f;
+      if (p.sink != nullptr) {
+        const float sk = p.sink[head] * 1.4426950408889634f, top = fmaxf(mm, sk);
+        f = exp2_fast(mm - top);
+        ll = fmaf(ll, f, exp2_fast(sk - top));
+      }
+      return ll == 0.f ? 0.f : f / ll;                // (a sequence without a visible key: zeros)
+    };
+    uint2 raw[HD / 64];                               // a thread's numbers of the queries that come next
+    auto fetch = [&](int head, int b) {
+      const int g0 = head % p.n_gchunks * DE_GM, g = st >> 4, part = st & 15;
+#pragma unroll
+      for (int k = 0; k < HD / 64; ++k) {
+        raw[k] = make_uint2(0u, 0u);
+        if (head < heads && g < min(GM, G - g0))
+          raw[k] = __ldcg(reinterpret_cast<const uint2*>(p.q + (size_t)b * p.ldq + (size_t)(head / p.n_gchunks * G + g0 + g) * HD + part * (HD / 16) + 4 * k));
+      }
+    };
+    auto prepare = [&](int buf) {
       const int g = st >> 4, part = st & 15;
       constexpr int N = HD / 16;
       float v[N];
       float most = 0.f;
 #pragma unroll
       for (int k = 0; k < N; k += 4) {
-        uint2 u = make_uint2(0u, 0u);
-        if (g < GC) u = __ldcg(reinterpret_cast<const uint2*>(p.q + (size_t)x.b * p.ldq + (size_t)(head0 + g) * HD + part * N + k));
+        const uint2 u = raw[k / 4];
         v[k] = __uint_as_float(u.x << 16);
         v[k + 1] = __uint_as_float(u.x & 0xffff0000u);
         v[k + 2] = __uint_as_float(u.y << 16);
@@ -484,9 +503,13 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       if (lane == 0) mbar_arrive(&q_full[buf]);
     };
     DecPlace at = start;
-    if (n_tiles > 0) prepare(at, 0);
+    if (n_tiles > 0) {
+      fetch(at.head, at.b);
+      prepare(0);
+    }
+    if (st < 2) shared_s[4 * st + 3] = 0;
     soft_sync();
-    int seg = 0, k_first = 0;
+    int seg = 0, k_first = 0, before[2] = {0, 0};
     bool fresh = true;
     float m[GM], l[GM], N[GM], n_t[GM], o[GM], fs[GM];
     int g0 = 0, GC = 0, head0 = 0, first_key = 0, last_key = 0;       // of the sequence
@@ -522,6 +545,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
         last_key = pos_s[at.b];
         key = (first_key / E8_PAGE + 2 * H * at.k) * E8_PAGE + r;
         k_first = at.k;
+        fetch(at.b + 1 < B ? at.head : at.head + 1, at.b + 1 < B ? at.b + 1 : 0);
 #pragma unroll
         for (int g = 0; g < GM; ++g) {
           m[g] = N[g] = n_t[g] = -1e30f;
@@ -529,7 +553,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
           fs[g] = fs_s[(seg & 1) * DE_GM + g];
         }
       }
-      if (ends && it + 1 < n_tiles) prepare(next, (seg + 1) & 1);
+      if (ends && it + 1 < n_tiles) prepare((seg + 1) & 1);
       wait(&sc_full[it % DE_SC], it / DE_SC);
       int kb[H], vb[H];
 #pragma unroll
@@ -661,112 +685,116 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
           }
 #pragma unroll
         for (int x = GM; x < 32; x <<= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
-        if (lane < GM) {
-          int g = 0;
+        int mine = 0;                                 // the head whose sum this lane has
 #pragma unroll
-          for (int x = 1, n = GM / 2; n > 0; x <<= 1, n >>= 1) g += (lane & x) ? n : 0;
-          ml_s[g * 4 + quarter] = make_float2(mw[0], l[0]);
-        }
+        for (int x = 1, n = GM / 2; n > 0; x <<= 1, n >>= 1) mine += (lane & x) ? n : 0;
+        if (lane < GM) ml_s[mine * 4 + quarter] = make_float2(mw[0], l[0]);
         soft_sync();
-        const size_t part0 = ((size_t)blockIdx.x * 2 + (k_first == 0 ? 1 : 0)) * GM;      // (a block shares two at most)
+        const int side = k_first == 0 ? 1 : 0;        // (a block shares two sequences at most: one that began before, one after)
+        const size_t part0 = ((size_t)blockIdx.x * 2 + side) * GM;
 #pragma unroll
         for (int g = 0; g < GM; ++g) {
           if (g >= GC) continue;
           const float2 w0 = ml_s[g * 4], w1 = ml_s[g * 4 + 1], w2 = ml_s[g * 4 + 2], w3 = ml_s[g * 4 + 3];
-          m[g] = fmaxf(fmaxf(w0.x, w1.x), fmaxf(w2.x, w3.x));
-          float ll = fmaf(w0.y, exp2_fast(w0.x - m[g]), w1.y * exp2_fast(w1.x - m[g])) +
-                     fmaf(w2.y, exp2_fast(w2.x - m[g]), w3.y * exp2_fast(w3.x - m[g]));
+          const float mm = fmaxf(fmaxf(w0.x, w1.x), fmaxf(w2.x, w3.x));
+          const float ll = fmaf(w0.y, exp2_fast(w0.x - mm), w1.y * exp2_fast(w1.x - mm)) +
+                           fmaf(w2.y, exp2_fast(w2.x - mm), w3.y * exp2_fast(w3.x - mm));
           // relative to m (in two steps: the values' powers may be far from the weights')
-          const float half = exp2_fast(0.5f * (N[g] - 8.f - m[g])), x = o[g] * half * half;
+          const float half = exp2_fast(0.5f * (N[g] - 8.f - mm)), x = o[g] * half * half;
           if (whole) {
-            float f = 1.f;
-            if (p.sink != nullptr) {
-              const float sk = p.sink[head0 + g] * 1.4426950408889634f, top = fmaxf(m[g], sk);
-              f = exp2_fast(m[g] - top);
-              ll = fmaf(ll, f, exp2_fast(sk - top));
-            }
-            f = ll == 0.f ? 0.f : f / ll;             // (a sequence without a visible key: zeros)
+            const float f = finish(head0 + g, mm, ll);
             if (has_dim) p.out[(size_t)at.b * p.ldo + (size_t)(head0 + g) * HD + dim] = __float2bfloat16_rn(x * f);
           } else {
             if (has_dim) p.part_acc[(part0 + g) * HD + dim] = x;
-            if (st == 0) *reinterpret_cast<float2*>(p.part_ml + (part0 + g) * 2) = make_float2(m[g], ll);
+            if (st == 0) *reinterpret_cast<float2*>(p.part_ml + (part0 + g) * 2) = make_float2(mm, ll);
           }
         }
         if (!whole) {
+          // This block's part is written; its ticket now, and whether that is the last when the block's run is over.
           soft_sync();
-          const long long unit = (long long)at.head * P + first[at.b];
-          const int i0 = block_of(unit), parts = block_of(unit + (at.nk == 1 ? 0 : at.nk)) - i0 + 1;
           if (st == 0) {
             // releases the block's part, which is behind the barrier; acquires those of the blocks before it for the
-            // other threads, behind the next one
+            // other threads, behind a later one
             int* ticket = p.tickets + (size_t)at.b * heads + at.head;
-            int before;
-            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
-            last = before == parts - 1;
-            if (before == parts - 1) *ticket = 0;     // for the next launch
-          }
-          soft_sync();
-          if (last) {
-            // a thread per four numbers, or 2, 4, 8 threads that share the parts; eight parts in flight each (four where registers are short)
-            const int cols = GC * H4;
-            int tpc = 1;
-            while (tpc < 8 && cols * tpc * 2 <= DE_SOFT) tpc *= 2;
-            for (int c0 = 0; c0 < cols; c0 += DE_SOFT / tpc) {
-              const int col = c0 + st / tpc;
-              const int g = min(col, cols - 1) / H4, d = min(col, cols - 1) % H4 * 4;
-              float mm = -1e30f, ll = 0.f;
-              float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-              for (int k0 = st % tpc; k0 < parts; k0 += JN * tpc) {
-                float2 ml[JN];
-                float4 v[JN];
-#pragma unroll
-                for (int j = 0; j < JN; ++j) {
-                  const int k = k0 + j * tpc;
-                  const size_t x = ((size_t)(i0 + min(k, parts - 1)) * 2 + (k == 0 ? 1 : 0)) * GM + g;
-                  ml[j] = k < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + x) : make_float2(-1e30f, 0.f);
-                  v[j] = k < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_acc + x * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-                float top = mm;
-#pragma unroll
-                for (int j = 0; j < JN; ++j) top = fmaxf(top, ml[j].x);
-                const float keep = exp2_fast(mm - top);
-                mm = top;
-                ll *= keep; a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
-#pragma unroll
-                for (int j = 0; j < JN; ++j) {
-                  const float w = exp2_fast(ml[j].x - top);
-                  ll = fmaf(w, ml[j].y, ll);
-                  a.x = fmaf(w, v[j].x, a.x); a.y = fmaf(w, v[j].y, a.y);
-                  a.z = fmaf(w, v[j].z, a.z); a.w = fmaf(w, v[j].w, a.w);
-                }
-              }
-              for (int x = tpc >> 1; x > 0; x >>= 1) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, mm, x), top = fmaxf(mm, m2);
-                const float k1 = exp2_fast(mm - top), k2 = exp2_fast(m2 - top);
-                mm = top;
-                ll = ll * k1 + __shfl_xor_sync(0xffffffffu, ll, x) * k2;
-                a.x = a.x * k1 + __shfl_xor_sync(0xffffffffu, a.x, x) * k2;
-                a.y = a.y * k1 + __shfl_xor_sync(0xffffffffu, a.y, x) * k2;
-                a.z = a.z * k1 + __shfl_xor_sync(0xffffffffu, a.z, x) * k2;
-                a.w = a.w * k1 + __shfl_xor_sync(0xffffffffu, a.w, x) * k2;
-              }
-              if (col < cols && st % tpc == 0) {
-                float f = 1.f;
-                if (p.sink != nullptr) {
-                  const float sk = p.sink[head0 + g] * 1.4426950408889634f, top = fmaxf(mm, sk);
-                  f = exp2_fast(mm - top);
-                  ll = fmaf(ll, f, exp2_fast(sk - top));
-                }
-                f = ll == 0.f ? 0.f : f / ll;
-                *reinterpret_cast<uint2*>(p.out + (size_t)at.b * p.ldo + (size_t)(head0 + g) * HD + d) =
-                    make_uint2(bf16_word(a.x * f, a.y * f), bf16_word(a.z * f, a.w * f));
-              }
-            }
+            int was;
+            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(was) : "l"(ticket) : "memory");
+            before[0] = side == 0 ? was : before[0];
+            before[1] = side == 1 ? was : before[1];
+            const long long unit = (long long)at.head * P + first[at.b];
+            const int i0 = block_of(unit);
+            shared_s[4 * side] = at.head;
+            shared_s[4 * side + 1] = at.b;
+            shared_s[4 * side + 2] = i0;
+            shared_s[4 * side + 3] = block_of(unit + (at.nk == 1 ? 0 : at.nk)) - i0 + 1;
           }
         }
         ++seg;
       }
       at = next;
+    }
+    soft_sync();
+    if (st == 0) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int parts = shared_s[4 * k + 3];
+        last_s[k] = parts > 0 && before[k] == parts - 1;
+        if (last_s[k]) p.tickets[(size_t)shared_s[4 * k + 1] * heads + shared_s[4 * k]] = 0;       // for the next launch
+      }
+    }
+    soft_sync();
+    for (int side = 0; side < 2; ++side) {
+      if (!last_s[side]) continue;                    // (block-uniform)
+      const int head = shared_s[4 * side], b = shared_s[4 * side + 1], i0 = shared_s[4 * side + 2], parts = shared_s[4 * side + 3];
+      const int first_head = head / p.n_gchunks * G + head % p.n_gchunks * DE_GM;
+      // a thread per four numbers, or 2, 4, 8 threads that share the parts; several parts in flight each
+      const int cols = min(GM, G - head % p.n_gchunks * DE_GM) * H4;
+      int tpc = 1;
+      while (tpc < 8 && cols * tpc * 2 <= DE_SOFT) tpc *= 2;
+      for (int c0 = 0; c0 < cols; c0 += DE_SOFT / tpc) {
+        const int col = c0 + st / tpc;
+        const int g = min(col, cols - 1) / H4, d = min(col, cols - 1) % H4 * 4;
+        float mm = -1e30f, ll = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k0 = st % tpc; k0 < parts; k0 += JN * tpc) {
+          float2 ml[JN];
+          float4 v[JN];
+#pragma unroll
+          for (int j = 0; j < JN; ++j) {
+            const int k = k0 + j * tpc;
+            const size_t x = ((size_t)(i0 + min(k, parts - 1)) * 2 + (k == 0 ? 1 : 0)) * GM + g;
+            ml[j] = k < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + x) : make_float2(-1e30f, 0.f);
+            v[j] = k < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_acc + x * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+          float top = mm;
+#pragma unroll
+          for (int j = 0; j < JN; ++j) top = fmaxf(top, ml[j].x);
+          const float keep = exp2_fast(mm - top);
+          mm = top;
+          ll *= keep; a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
+#pragma unroll
+          for (int j = 0; j < JN; ++j) {
+            const float w = exp2_fast(ml[j].x - top);
+            ll = fmaf(w, ml[j].y, ll);
+            a.x = fmaf(w, v[j].x, a.x); a.y = fmaf(w, v[j].y, a.y);
+            a.z = fmaf(w, v[j].z, a.z); a.w = fmaf(w, v[j].w, a.w);
+          }
+        }
+        for (int x = tpc >> 1; x > 0; x >>= 1) {
+          const float m2 = __shfl_xor_sync(0xffffffffu, mm, x), top = fmaxf(mm, m2);
+          const float k1 = exp2_fast(mm - top), k2 = exp2_fast(m2 - top);
+          mm = top;
+          ll = ll * k1 + __shfl_xor_sync(0xffffffffu, ll, x) * k2;
+          a.x = a.x * k1 + __shfl_xor_sync(0xffffffffu, a.x, x) * k2;
+          a.y = a.y * k1 + __shfl_xor_sync(0xffffffffu, a.y, x) * k2;
+          a.z = a.z * k1 + __shfl_xor_sync(0xffffffffu, a.z, x) * k2;
+          a.w = a.w * k1 + __shfl_xor_sync(0xffffffffu, a.w, x) * k2;
+        }
+        if (col < cols && st % tpc == 0) {
+          const float f = finish(first_head + g, mm, ll);
+          *reinterpret_cast<uint2*>(p.out + (size_t)b * p.ldo + (size_t)(first_head + g) * HD + d) =
+              make_uint2(bf16_word(a.x * f, a.y * f), bf16_word(a.z * f, a.w * f));
+        }
+      }
     }
   }
 
