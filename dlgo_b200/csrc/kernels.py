@@ -2700,7 +2700,8 @@ def decode_layers(desc: torch.Tensor, n_layers: int, residual: torch.Tensor, hid
 
 # ------------------------------------------------------------------ the layer loop of a prompt step, native
 class PromptEntryPoints(ctypes.Structure):
-    _fields_ = [(n, _p) for n in ("rmsnorm", "gemm_tc", "rope_append", "attention", "gemm_tc_rope", "gemm_tc_stream")]
+    _fields_ = [(n, _p) for n in ("rmsnorm", "gemm_tc", "rope_append", "attention", "gemm_tc_rope", "gemm_tc_stream", "write_e4m3",
+                                  "read_e4m3")]
 
 
 class PromptShape(ctypes.Structure):
@@ -2710,46 +2711,60 @@ class PromptShape(ctypes.Structure):
 
 class PromptLayer(ctypes.Structure):
     _fields_ = [("w_qkv", _p), ("w_o", _p), ("w_gate_up", _p), ("w_down", _p), ("norm1_w", _p), ("norm2_w", _p),
-                ("eps1", _f), ("eps2", _f), ("kpages", _p), ("vpages", _p), ("n_pages", _i), ("write_cache", _i)]
+                ("eps1", _f), ("eps2", _f), ("kpages", _p), ("vpages", _p), ("n_pages", _i), ("write_cache", _i),
+                ("kscales", _p), ("vscales", _p)]
 
 
 class PromptStep(ctypes.Structure):
     _fields_ = [("tokens", _i), ("residual", _p), ("x", _p), ("qkv", _p), ("attn_out", _p), ("h", _p), ("cos_t", _p),
                 ("sin_t", _p), ("token_pos", _p), ("token_seq", _p), ("seq_slot", _p), ("page_table", _p),
                 ("max_pages", _i), ("tiles", _p), ("n_tiles", _i), ("bn", _i * 4), ("pair", _i * 4), ("fuse_rope", _i),
-                ("form", _i * 4), ("splits", _i * 4), ("qkv_sum", _p)]
+                ("form", _i * 4), ("splits", _i * 4), ("qkv_sum", _p), ("q", _p), ("n_positions", _i), ("n_slots", _i), ("seen", _p),
+                ("n_seen", _i), ("seen_table", _p), ("seen_width", _i), ("seen_rows", _p), ("keys", _p), ("values", _p)]
 
 
-PROMPT_CALLS = ("mixer norm", "q/k/v projection", "rotation and cache append (0 launches where the projection does it)", "attention", "output projection",
+PROMPT_CALLS = ("mixer norm", "q/k/v projection", "rotation and cache append (0 launches where the projection does it; with an 8-bit cache also the pages' "
+                "way back)", "attention", "output projection",
                 "feed-forward norm", "gate/up projection", "down projection")
 
 
-def prompt_entry_points() -> PromptEntryPoints:
+def prompt_entry_points(e4m3: bool = False) -> PromptEntryPoints:
     """Addresses of the entry points that the native layer loop calls (their libraries are loaded, and
-    compiled first if need be)."""
+    compiled first if need be); ``e4m3``: with those of the 8-bit cache."""
     def address(lib: str, fn: str) -> int:
         return ctypes.cast(getattr(_lib(lib), fn), ctypes.c_void_p).value
     return PromptEntryPoints(address("elementwise", "dlgo_rmsnorm"), address("gemm_tc", "dlgo_gemm_tc"),
                              address("rope_append", "dlgo_rope_append"),
                              address("attention_prefill_tc", "dlgo_attention_prefill_tc"),
-                             address("gemm_tc", "dlgo_gemm_tc_rope"), address("gemm_tc", "dlgo_gemm_tc_stream"))
+                             address("gemm_tc", "dlgo_gemm_tc_rope"), address("gemm_tc", "dlgo_gemm_tc_stream"),
+                             *((address("cache_e4m3", "dlgo_write_e4m3"), address("cache_e4m3", "dlgo_read_e4m3")) if e4m3 else ()))
 
 
 def prompt_layers_describe(layers: Sequence[dict]) -> tuple:
     """The host-side descriptor array of a run of layers: (ctypes array, the tensors it points at, which the
     caller keeps alive with it).  Each entry gives ``w_qkv, w_o, w_gate_up, w_down`` (bfloat16, contiguous),
-    ``norm1_w, norm2_w`` (float32), ``kpages, vpages`` (bfloat16) and ``eps1, eps2, write_cache``."""
+    ``norm1_w, norm2_w`` (float32), ``kpages, vpages`` (bfloat16; or e4m3, with ``kscales, vscales``) and ``eps1, eps2,
+    write_cache``."""
     arr = (PromptLayer * len(layers))()
     keep = []
     for i, L in enumerate(layers):
-        for n in ("w_qkv", "w_o", "w_gate_up", "w_down", "kpages", "vpages"):
+        e4m3 = L.get("kscales") is not None
+        for n in ("w_qkv", "w_o", "w_gate_up", "w_down"):
             _need(L[n], torch.bfloat16, n)
+        for n in ("kpages", "vpages"):
+            _need(L[n], _E8 if e4m3 else torch.bfloat16, n)
         for n in ("norm1_w", "norm2_w"):
             _need(L[n], torch.float32, n)
         a = arr[i]
         for n in ("w_qkv", "w_o", "w_gate_up", "w_down", "norm1_w", "norm2_w", "kpages", "vpages"):
             setattr(a, n, L[n].data_ptr())
             keep.append(L[n])
+        if e4m3:
+            _check_e4m3("prompt_layers", L["kpages"], L["vpages"], L["kscales"], L["vscales"], L["page_table"])
+            for n in ("kscales", "vscales"):
+                _need(L[n], torch.uint8, n)
+                setattr(a, n, L[n].data_ptr())
+                keep.append(L[n])
         a.eps1, a.eps2 = L["eps1"], L["eps2"]
         a.n_pages, a.write_cache = L["kpages"].shape[0], 1 if L["write_cache"] else 0
     return arr, keep
@@ -2757,7 +2772,7 @@ def prompt_layers_describe(layers: Sequence[dict]) -> tuple:
 
 def prompt_layers(entry: PromptEntryPoints, shape: PromptShape, layers: ctypes.Array, step: PromptStep) -> None:
     """Run ``len(layers)`` pre-norm layers of a prompt step: eight launches a layer (seven where the q/k/v
-    projection rotates and appends in its epilogue: ``step.fuse_rope``), issued from one native loop
+    projection rotates and appends in its epilogue: ``step.fuse_rope``; nine over an 8-bit cache), issued from one native loop
     (csrc/prompt_layers.cu).  The caller has checked types and sizes of what ``step`` points at."""
     failed = _i(-1)
     n = len(layers)
@@ -2765,4 +2780,4 @@ def prompt_layers(entry: PromptEntryPoints, shape: PromptShape, layers: ctypes.A
                                                   ctypes.byref(step), ctypes.byref(failed), _stream())
     if st != 0 and failed.value >= 0:
         _check(st, f"prompt_layers (layer {failed.value // 8} of the run, {PROMPT_CALLS[failed.value % 8]})")
-    _check(st, "prompt_layers", (7 if step.fuse_rope else 8) * n)
+    _check(st, "prompt_layers", (7 if step.fuse_rope else 9 if n and layers[0].kscales else 8) * n)

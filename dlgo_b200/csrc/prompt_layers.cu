@@ -31,6 +31,14 @@ typedef int (*AttentionFn)(const void* q, int T, int ldq, const void* kpages, co
                            const int* token_pos, void* out, int ldo, int Hq, int Hkv, int hd, int window, float scale, const float* sink, int split,
                            cudaStream_t stream);
 
+typedef int (*WriteE4m3Fn)(void* qkv, int dtype, int T, int ld, const float* cos_t, const float* sin_t, int n_positions,
+                           const int* token_pos, const int* token_seq, const int* seq_slot, const int* page_table, int n_slots,
+                           int max_pages, void* kpages, void* vpages, void* kscales, void* vscales, int n_pages, void* q, int Hq, int Hkv,
+                           int hd, int rot, int interleaved, int write_cache, int clear, cudaStream_t stream);
+typedef int (*ReadE4m3Fn)(const void* kpages, const void* vpages, const void* kscales, const void* vscales, int n_pages,
+                          const int* page_table, int n_slots, int max_pages, const int* pages, int n, void* keys, void* values, int Hkv,
+                          int hd, cudaStream_t stream);
+
 // as in gemm_tc.cu
 struct DlgoRopeArgs {
   const float* cos_t;
@@ -58,6 +66,8 @@ struct DlgoPromptEntryPoints {
   AttentionFn attention;
   GemmTcRopeFn gemm_tc_rope;
   GemmTcStreamFn gemm_tc_stream;
+  WriteE4m3Fn write_e4m3;       // (the last two: null where the cache is not kept in 8 bits)
+  ReadE4m3Fn read_e4m3;
 };
 
 // What the layers of a run share.
@@ -80,6 +90,8 @@ struct DlgoPromptLayer {
   void* vpages;
   int n_pages;
   int write_cache;
+  void* kscales;          // the 8-bit cache's scale bytes; null: bfloat16 pages
+  void* vscales;
 };
 
 // One step: the residual stream, buffers for the layers' intermediates, the batch's tables, and the tile
@@ -107,6 +119,18 @@ struct DlgoPromptStep {
                           // tile, `splits` K-slices), 2 the weight streamed by persistent CTAs (added into fp32)
   int splits[4];
   float* qkv_sum;         // forms 1 and 2: [tokens, (heads + 2 kv_heads) * head_dim] fp32, zero; left zero
+  // The 8-bit cache: rotated queries go to q, and the pages that the step's queries see are read back as bfloat16 before
+  // attention reads them there.
+  void* q;                // [tokens, heads * head_dim] bf16
+  int n_positions;        // rows of cos_t and sin_t
+  int n_slots;            // rows of page_table
+  const int* seen;        // [n_seen][3] (slot, page of its sequence, rows)
+  int n_seen;
+  const int* seen_table;  // [sequences][seen_width] a sequence's pages in that list
+  int seen_width;
+  const int* seen_rows;   // [sequences] their rows of seen_table
+  void* keys;             // [n_seen][kv_heads][page_size][head_dim] bf16
+  void* values;
 };
 
 }  // extern "C"
@@ -124,6 +148,8 @@ DLGO_EXPORT int dlgo_prompt_layers(const DlgoPromptEntryPoints* fn, const DlgoPr
   if (fn->rmsnorm == nullptr || fn->gemm_tc == nullptr || fn->rope_append == nullptr || fn->attention == nullptr ||
       fn->gemm_tc_rope == nullptr || fn->gemm_tc_stream == nullptr)
     return DLGO_ERR_DRIVER;
+  const bool e8 = n_layers > 0 && layers[0].kscales != nullptr;
+  if (e8 && (fn->write_e4m3 == nullptr || fn->read_e4m3 == nullptr)) return DLGO_ERR_DRIVER;
   const int T = p->tokens, d = s->hidden;
   const int q_dim = s->heads * s->head_dim, n_cols = (s->heads + 2 * s->kv_heads) * s->head_dim;
   if (T <= 0 || n_layers <= 0) return DLGO_OK;
@@ -150,7 +176,22 @@ DLGO_EXPORT int dlgo_prompt_layers(const DlgoPromptEntryPoints* fn, const DlgoPr
     const DlgoPromptLayer& L = layers[l];
     call = 8 * l;
     DLGO_STEP(fn->rmsnorm(p->residual, L.norm1_w, p->x, DLGO_BF16, nullptr, T, d, L.eps1, stream));
-    if (p->fuse_rope) {
+    if (e8) {
+      const bool sum = p->form[0] != 0;
+      if (p->fuse_rope || L.kscales == nullptr || (sum && p->qkv_sum == nullptr)) return DLGO_ERR_SIZE;
+      void* proj = sum ? (void*)p->qkv_sum : p->qkv;
+      DLGO_STEP(product(0, p->x, L.w_qkv, n_cols, d, proj, n_cols, sum ? TC_ADD_F32 : TC_STORE));
+      st = fn->write_e4m3(proj, sum ? DLGO_F32 : DLGO_BF16, T, n_cols, p->cos_t, p->sin_t, p->n_positions, p->token_pos, p->token_seq,
+                          p->seq_slot, p->page_table, p->n_slots, p->max_pages, L.kpages, L.vpages, L.kscales, L.vscales, L.n_pages, p->q,
+                          s->heads, s->kv_heads, s->head_dim, s->rotary_dim, s->interleaved, L.write_cache, sum ? 1 : 0, stream);
+      if (st == DLGO_OK)
+        st = fn->read_e4m3(L.kpages, L.vpages, L.kscales, L.vscales, L.n_pages, p->page_table, p->n_slots, p->max_pages, p->seen,
+                           p->n_seen, p->keys, p->values, s->kv_heads, s->head_dim, stream);
+      DLGO_STEP(st);
+      DLGO_STEP(fn->attention(p->q, T, q_dim, p->keys, p->values, p->n_seen, p->seen_table, p->seen_width, p->tiles, p->n_tiles,
+                              p->seen_rows, p->token_pos, p->attn_out, q_dim, s->heads, s->kv_heads, s->head_dim, s->window, s->scale,
+                              nullptr, 0, stream));
+    } else if (p->fuse_rope) {
       const DlgoRopeArgs rope = {p->cos_t, p->sin_t, p->token_pos, p->token_seq, p->seq_slot, p->page_table,
                                  p->max_pages, L.kpages, L.vpages, s->heads, s->kv_heads, s->head_dim, L.write_cache};
       DLGO_STEP(fn->gemm_tc_rope(p->x, T, d, L.w_qkv, n_cols, d, d, p->qkv, n_cols, p->pair[0], &rope, stream));
@@ -164,9 +205,10 @@ DLGO_EXPORT int dlgo_prompt_layers(const DlgoPromptEntryPoints* fn, const DlgoPr
                                 s->head_dim, s->rotary_dim, s->page_size, s->interleaved, L.write_cache,
                                 sum ? p->qkv_sum : nullptr, sum ? 1 : 0, 0, sum ? 1 : 0, stream));
     }
-    DLGO_STEP(fn->attention(p->qkv, T, n_cols, L.kpages, L.vpages, L.n_pages, p->page_table, p->max_pages, p->tiles,
-                            p->n_tiles, p->seq_slot, p->token_pos, p->attn_out, q_dim, s->heads, s->kv_heads,
-                            s->head_dim, s->window, s->scale, nullptr, 0, stream));
+    if (!e8)
+      DLGO_STEP(fn->attention(p->qkv, T, n_cols, L.kpages, L.vpages, L.n_pages, p->page_table, p->max_pages, p->tiles,
+                              p->n_tiles, p->seq_slot, p->token_pos, p->attn_out, q_dim, s->heads, s->kv_heads,
+                              s->head_dim, s->window, s->scale, nullptr, 0, stream));
     DLGO_STEP(product(1, p->attn_out, L.w_o, d, q_dim, p->residual, d, TC_ADD_F32));
     DLGO_STEP(fn->rmsnorm(p->residual, L.norm2_w, p->x, DLGO_BF16, nullptr, T, d, L.eps2, stream));
     DLGO_STEP(product(2, p->x, L.w_gate_up, 2 * s->ffn, d, p->h, s->ffn, TC_SWIGLU));

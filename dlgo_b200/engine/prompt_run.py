@@ -45,6 +45,11 @@ STREAM_MAX = min(K.GEMM_TC_STREAM_MAX, int(os.environ.get("DLGO_PROMPT_STREAM_MA
 ENABLED = os.environ.get("DLGO_NATIVE_PROMPT", "1") != "0"
 
 
+def _is_e4m3(view: Any) -> bool:
+    """Whether a cache's view holds 8-bit rows with scale bytes."""
+    return getattr(view, "key_scales", None) is not None
+
+
 def _signature(blk: Any, positions: Dict[str, Any]) -> Optional[tuple]:
     """What two blocks must share to run in one native loop, or ``None`` if the loop does not take the block."""
     if type(blk) is not PreNormBlock:
@@ -84,7 +89,8 @@ class PromptRun:
         sums = attention._QKV_SUM and not tensor_core.ORDERED_SUMS and ctx.n_tokens <= tensor_core.RED_MAX_TOKENS
         return (not ctx.decode and view is not None and (sums or not few) and
                 K._profile_events is None and
-                K.attention_prefill_tc_takes(torch.bfloat16, hd, view.page_size) and view.keys.dtype == torch.bfloat16)
+                K.attention_prefill_tc_takes(torch.bfloat16, hd, view.page_size) and
+                (view.keys.dtype == torch.bfloat16 or _is_e4m3(view)))
 
     def _descriptors(self, model: Any, cache: Any) -> tuple:
         hit = self._layers.get(id(cache))
@@ -99,7 +105,7 @@ class PromptRun:
                     w_qkv=blk.mixer.wqkv.weight, w_o=blk.mixer.wo.weight, w_gate_up=blk.ffn.w_gate_up.weight,
                     w_down=blk.ffn.w_down.weight, norm1_w=blk.mixer_norm.weight, norm2_w=blk.ffn_norm.weight,
                     eps1=blk.mixer_norm.eps, eps2=blk.ffn_norm.eps, kpages=view.keys, vpages=view.values,
-                    write_cache=view.writes))
+                    kscales=view.key_scales, vscales=view.value_scales, page_table=view.page_table, write_cache=view.writes))
             hit = self._layers[id(cache)] = (weakref.ref(cache),) + K.prompt_layers_describe(layers)
         return hit[1], hit[2]
 
@@ -110,8 +116,9 @@ class PromptRun:
         blk = model.blocks[model.order[self.first].layer]
         if residual.dtype != torch.float32 or not residual.is_contiguous() or tuple(residual.shape) != (T, d):
             raise K.KernelError("the residual stream must be contiguous float32 [tokens, hidden]")
+        e4m3 = _is_e4m3(view)
         if self._entry is None:
-            self._entry = K.prompt_entry_points()
+            self._entry = K.prompt_entry_points(True) if e4m3 else K.prompt_entry_points()
         layers, _keep = self._descriptors(model, cache)
         if pe_name is not None:
             pe = model.positions[pe_name]
@@ -145,6 +152,14 @@ class PromptRun:
                     step.form[j] = 2
         if step.form[0] != 0:
             step.qkv_sum = ctx.zeros(f"qkv_sum{n_cols}", T * n_cols, torch.float32).data_ptr()
+        if e4m3:
+            seen, table, at = ctx.pages_in_sight(window, view.page_size)
+            n = seen.shape[0] * hkv * view.page_size * hd
+            step.q = ctx.scratch("prompt_q", T * hq * hd, torch.bfloat16).data_ptr()
+            step.n_positions, step.n_slots = (cos.shape[0] if rot else 0), view.page_table.shape[0]
+            step.seen, step.n_seen = seen.data_ptr(), seen.shape[0]
+            step.seen_table, step.seen_width, step.seen_rows = table.data_ptr(), table.shape[1], at.data_ptr()
+            step.keys, step.values = (ctx.scratch(f"attention_e4m3_{name}", n, torch.bfloat16).data_ptr() for name in ("keys", "values"))
         step.fuse_rope = 1 if step.form[0] == 0 and pe_name is not None and blk.mixer.fuses_prompt_rope(ctx, view, model.positions) else 0
         shape = K.PromptShape(d, hq, hkv, hd, f, rot, 1 if inter else 0, window, view.page_size, scale)
         K.prompt_layers(self._entry, shape, layers, step)

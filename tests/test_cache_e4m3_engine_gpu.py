@@ -168,6 +168,19 @@ def test_requests_in_pieces_and_single_tokens_among_prompts(name, mixed):
     check(name, steps, T.run_in_process(engine(name, True, mixed), steps), reqs, mixed)
 
 
+@pytest.mark.parametrize("name", list(SIZES))
+def test_prompts_part_by_part(name, monkeypatch):
+    """The other tests' prompts go through the native loop over the layers; here every part runs by itself.  (Two runs of either
+    kind may differ by twice what each is off: their few-token products add their slices in any order, and a key that lies near a
+    border between two e4m3 numbers then falls on its other side.)"""
+    eng = engine(name)
+    assert eng.model.prompt_runs
+    reqs = requests(name)
+    monkeypatch.setattr(eng.model, "prompt_runs", {})
+    for steps in (T.whole(reqs), T.chunked(reqs, [30, 70, 200])):
+        check(name, steps, T.run_in_process(eng, steps), reqs)
+
+
 def test_ordered_sums_run_too(tmp_path):
     """K-slices kept apart (a setting of the process): the projection then comes finished, not as a sum to be cleared."""
     import os
