@@ -459,3 +459,101 @@ def test_a_sequence_grows_token_by_token_through_a_captured_step(hq, hkv, hd):
                 _check_decode(out, want, hd, hq // hkv)
     torch.cuda.current_stream().wait_stream(stream)
     K().check_device_errors()
+
+
+# ------------------------------------------------------------------ calls that users may make
+def test_decode_on_two_streams_at_once():
+    """Two launches with workspaces of their own, on two streams, many times over."""
+    cases = [_decode_case(8, 2, 64, [3000, 700, 64, 1]), _decode_case(16, 2, 128, [2500, 1, 130])]
+    want = [K().attention_decode_e4m3(*a, **m).clone() for a, m, _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(30):
+        for i, (a, m, _) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(K().attention_decode_e4m3(*a, **m))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+    K().check_device_errors()
+
+
+def test_decode_launches_one_behind_another_share_their_workspaces():
+    """Launches of other lengths and sizes with the same scratch and tickets, without a pause in between."""
+    cases = [_decode_case(8, 2, 128, lens) for lens in ([4000], [1, 2, 3], [700] * 9, [64, 2000])]
+    want = [K().attention_decode_e4m3(*a, **m).clone() for a, m, _ in cases]
+    scratch = torch.empty(K().attention_decode_e4m3_scratch(8, 2, 128), device=DEV)
+    tickets = torch.zeros(9 * 2, dtype=torch.int32, device=DEV)
+    outs = [[K().attention_decode_e4m3(*a, scratch=scratch, tickets=tickets, **m) for a, m, _ in cases] for _ in range(10)]
+    torch.cuda.synchronize()
+    for row in outs:
+        assert all(torch.equal(o, w) for o, w in zip(row, want))
+    assert (tickets == 0).all()
+
+
+def test_decode_of_one_sequence_several_times_and_of_pages_that_two_share():
+    hq, hkv, hd = 8, 2, 64
+    args, more, want = _decode_case(hq, hkv, hd, [300])
+    q = args[0].repeat(5, 1)
+    pos = [299, 0, 63, 64, 299]
+    cut = list(args)
+    cut[0], cut[6], cut[7] = q, args[6].repeat(5), ints(pos)
+    out = K().attention_decode_e4m3(*cut, **more)
+    assert torch.equal(out[0], out[4])
+    _check_decode(out[[0]], want, hd, hq // hkv)
+    k, v = (P.values(args[i], args[i + 2])[args[5][int(args[6][0]), :5].cpu().long()].transpose(1, 2).reshape(-1, hkv, hd) for i in (1, 2))
+    for j, p in enumerate(pos):
+        _check_decode(out[[j]], [P.attend(args[0][0].cpu().view(hq, hd), k[:p + 1], v[:p + 1], hd ** -0.5)], hd, hq // hkv)
+    # two sequences whose first pages are the same ones
+    table = args[5].clone()
+    other = int(args[6][0]) - 1
+    table[other] = table[int(args[6][0])]
+    cut = list(args)
+    cut[0], cut[5], cut[6], cut[7] = q[:2], table, ints([int(args[6][0]), other]), ints([299, 200])
+    out = K().attention_decode_e4m3(*cut, **more)
+    _check_decode(out, want + [P.attend(args[0][0].cpu().view(hq, hd), k[:201], v[:201], hd ** -0.5)], hd, hq // hkv)
+
+
+def test_numbers_outside_the_tables_reach_no_other_row():
+    """Slots, positions and page numbers that the tables do not have: kept within them; the other sequences' results stay."""
+    hq, hkv, hd = 8, 2, 64
+    args, more, want = _decode_case(hq, hkv, hd, [100, 400, 70])
+    for slot, pos in ((77, 50), (-3, 50), (int(args[6][1]), 1 << 30), (int(args[6][1]), -(1 << 30))):
+        cut = list(args)
+        cut[6], cut[7] = ints([int(args[6][0]), slot, int(args[6][2])]), ints([99, pos, 69])
+        out = K().attention_decode_e4m3(*cut, **more)
+        _check_decode(out[[0, 2]], [want[0], want[2]], hd, hq // hkv)
+    cut = list(args)
+    cut[5] = args[5].clone()
+    cut[5][int(args[6][1])] = torch.tensor([1 << 30, -5, 9999, -1] + [0] * 9, dtype=torch.int32)[:args[5].shape[1]]
+    out = K().attention_decode_e4m3(*cut, **more)
+    _check_decode(out[[0, 2]], [want[0], want[2]], hd, hq // hkv)
+    K().check_device_errors()
+
+
+def test_alignment_is_asked_for():
+    hq, hkv, hd = 8, 2, 64
+    args, more, _ = _decode_case(hq, hkv, hd, [100, 40])
+    odd = torch.zeros(2, hq * hd + 2, dtype=torch.bfloat16, device=DEV)
+    for q, out in ((odd[:, 1:hq * hd + 1], None), (odd[:, :hq * hd], None), (args[0], odd[:, 1:hq * hd + 1])):
+        with pytest.raises(K().KernelError, match="alignment"):
+            K().attention_decode_e4m3(q, *args[1:], out=out, **more)
+    buffer = torch.zeros(1 + args[1].numel(), dtype=torch.uint8, device=DEV)
+    shifted = buffer[1:].view(torch.float8_e4m3fn).view(args[1].shape)
+    with pytest.raises(K().KernelError, match="alignment"):
+        K().attention_decode_e4m3(args[0], shifted, *args[2:], **more)
+    with pytest.raises(K().KernelError, match="alignment"):
+        K().read_pages_e4m3(shifted, *args[2:6], torch.zeros(1, 3, dtype=torch.int32, device=DEV))
+    qkv = torch.zeros(2, (hq + 2 * hkv) * hd + 4, device=DEV)
+    cos = torch.zeros(64, 32, device=DEV)
+    with pytest.raises(K().KernelError, match="alignment"):
+        K().rope_append_e4m3(qkv[:, :-4], cos, cos, ints([0, 1]), ints([0, 0]), args[6], *args[1:6], hq, hkv, hd, hd)
+
+
+def test_nothing_to_do_is_done():
+    hq, hkv, hd = 8, 2, 64
+    args, _, _ = _decode_case(hq, hkv, hd, [100])
+    cos = torch.zeros(64, 32, device=DEV)
+    q = K().rope_append_e4m3(torch.zeros(0, (hq + 2 * hkv) * hd, device=DEV), cos, cos, ints([]), ints([]), args[6], *args[1:6], hq, hkv, hd, hd)
+    assert q.shape == (0, hq * hd)
