@@ -478,7 +478,9 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
       for (int o = 1; o < 16; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
       const int e = min(max((int)(__float_as_uint(most) >> 23), 8), 254);
-      const float down = __uint_as_float((unsigned)(261 - e) << 23);            // 2^(7 - (e - 127))
+      // 2^(7 - (e - 127)); NaN for a row with an infinity, whose scores the formula leaves without a value (the terms would hold it
+      // as 448)
+      const float down = __uint_as_float(most == INFINITY ? 0x7fc00000u : (unsigned)(261 - e) << 23);
       if (g < GM) {
         uint32_t hi[N / 4], lo4[N / 4];
 #pragma unroll

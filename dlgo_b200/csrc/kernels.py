@@ -1608,7 +1608,8 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
     """Attention of one new token per sequence over its rows of the 8-bit cache (its own key and value, at ``token_pos``,
     included): ``q`` [sequences, heads * head_dim] bfloat16 -> [sequences, heads * head_dim] bfloat16.  ``window``: as the other
     attention kernels take it (0: every key; w: keys t > pos - w; -c: chunks of c positions).  ``sink`` [heads] joins the
-    denominator.  A position of -1 sees nothing and gives zeros.  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
+    denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives
+    NaN.  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
     ``tickets`` (a zero int32 per sequence and chunk of 8 heads of a kv head, left zero) are made here when not given; given ones
     belong to one launch at a time."""
     what = "attention_decode_e4m3"

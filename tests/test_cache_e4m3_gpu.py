@@ -557,3 +557,15 @@ def test_nothing_to_do_is_done():
     cos = torch.zeros(64, 32, device=DEV)
     q = K().rope_append_e4m3(torch.zeros(0, (hq + 2 * hkv) * hd, device=DEV), cos, cos, ints([]), ints([]), args[6], *args[1:6], hq, hkv, hd, hd)
     assert q.shape == (0, hq * hd)
+
+
+def test_a_query_head_with_an_infinity_gives_nan_and_the_others_their_numbers():
+    for hq, hkv, hd in ((8, 2, 64), (8, 1, 128)):
+        args, more, want = _decode_case(hq, hkv, hd, [100, 700, 70])
+        q = args[0].view(3, hq, hd)
+        q[1, 2, 5], q[1, 5, 40], q[0, 3, 7] = float("inf"), -float("inf"), float("nan")
+        out = K().attention_decode_e4m3(*args, **more).view(3, hq, hd)
+        for i, h in ((1, 2), (1, 5), (0, 3)):
+            assert torch.isnan(out[i, h]).all()
+            out[i, h] = want[i][0].reshape(hq, hd)[h].to(out)
+        _check_decode(out.view(3, -1), want, hd, hq // hkv)
