@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 from typing import List, NamedTuple, Optional, Sequence
 
 import torch
@@ -1508,13 +1509,16 @@ def _e4m3_entry(lib: str, name: str, argtypes: str):
 
 def _on_device_of(fn):
     """Run with the first argument's device current, so that the launch goes to that device's current stream."""
+    name = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
-    def call(first: torch.Tensor, *args, **kwargs):
-        index = first.get_device()
+    def call(*args, **kwargs):
+        first = args[0] if args else kwargs.get(name)
+        index = first.get_device() if first is not None else -1
         if index < 0 or index == torch._C._cuda_getDevice():
-            return fn(first, *args, **kwargs)
+            return fn(*args, **kwargs)
         with torch.cuda.device(index):
-            return fn(first, *args, **kwargs)
+            return fn(*args, **kwargs)
     return call
 
 
@@ -1608,8 +1612,8 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
     """Attention of one new token per sequence over its rows of the 8-bit cache (its own key and value, at ``token_pos``,
     included): ``q`` [sequences, heads * head_dim] bfloat16 -> [sequences, heads * head_dim] bfloat16.  ``window``: as the other
     attention kernels take it (0: every key; w: keys t > pos - w; -c: chunks of c positions).  ``sink`` [heads] joins the
-    denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives
-    NaN.  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
+    denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives NaN.  ``out`` is
+    another tensor than ``q``.  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
     ``tickets`` (a zero int32 per sequence and chunk of 8 heads of a kv head, left zero) are made here when not given; given ones
     belong to one launch at a time."""
     what = "attention_decode_e4m3"
@@ -1622,6 +1626,8 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
         out = torch.empty_like(q) if q.shape[1] == cols and q.is_contiguous() else q.new_empty((B, cols))
     else:
         _need_rows(what, "out", out, B, cols)
+        if B > 0 and out.data_ptr() == q.data_ptr():       # (one block writes a head while another has yet to read its query)
+            raise KernelError(f"{what}: out must be another tensor than q")
     if seq_slot.numel() < B or token_pos.numel() < B:
         raise KernelError(f"{what}: a slot and a position per sequence")
     if sink is not None and sink.numel() != num_heads:

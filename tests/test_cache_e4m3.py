@@ -105,3 +105,12 @@ def test_pages_in_sight_of_a_step():
     assert pages.tolist()[1] == [2, 1, 64] and table.tolist()[1] == [-1, 1, 2, 3]
     pages, table, _ = ctx().pages_in_sight(-100, 64)        # chunks of 100: from position 100 on
     assert pages.tolist() == [[7, 0, 3], [2, 1, 64], [2, 2, 64], [2, 3, 3], [5, 0, 64]]
+
+
+def test_operators_take_their_arguments_by_name():
+    from dlgo_b200.csrc import kernels as K
+    kp, vp, ks, vs, pt = _tensors()
+    with pytest.raises(K.KernelError, match="GPU"):
+        K.read_pages_e4m3(kpages=kp, vpages=vp, kscales=ks, vscales=vs, page_table=pt, pages=torch.zeros(1, 3, dtype=torch.int32))
+    with pytest.raises(TypeError, match="kpages"):
+        K.read_pages_e4m3(vpages=vp)

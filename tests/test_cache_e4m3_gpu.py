@@ -569,3 +569,12 @@ def test_a_query_head_with_an_infinity_gives_nan_and_the_others_their_numbers():
             assert torch.isnan(out[i, h]).all()
             out[i, h] = want[i][0].reshape(hq, hd)[h].to(out)
         _check_decode(out.view(3, -1), want, hd, hq // hkv)
+
+
+def test_keywords_alone_and_an_output_in_the_queries_place():
+    hq, hkv, hd = 4, 2, 64
+    args, more, want = _decode_case(hq, hkv, hd, [100, 7])
+    names = ("q", "kpages", "vpages", "kscales", "vscales", "page_table", "seq_slot", "token_pos", "num_heads", "num_kv_heads", "head_dim", "scale")
+    _check_decode(K().attention_decode_e4m3(**dict(zip(names, args)), **more), want, hd, hq // hkv)
+    with pytest.raises(K().KernelError, match="another tensor"):
+        K().attention_decode_e4m3(*args, **more, out=args[0])
