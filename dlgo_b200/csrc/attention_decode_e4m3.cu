@@ -14,30 +14,40 @@
 //
 // Both products have e4m3 on both sides.  The other operand enters as several e4m3 terms in columns of their own: a query as
 // x = x1 + x2 / 16, which holds a bfloat16 number whole down to 2^-22 of the row's largest (each term keeps 4 bits, and what
-// the first leaves over is at most 2^-4 of it); a weight as w1 + w2 / 16 (+ w3 / 256 where a block has four heads at most):
-// 2^-8 (2^-11, passing through float16) of its size, and of the tile's largest weight 2^-22 (2^-26).  The values' powers are part of the weights, so a
-// row of small values may hold all of the softmax's weight without a loss; and because every tile has a reference of its
-// own, neither does a long tail of small weights behind a large one.
+// the first leaves over is at most 2^-4 of it); a weight as w1 + w2 / 16, 2^-8 of its size, or, where a block has four heads at
+// most and columns are left, + w3 / 256, 2^-11 (it passes through float16); and 2^-22 (2^-26) of the tile's largest weight.
+// The values' powers are part of the weights, so a row of small values may hold all of the softmax's weight without a loss;
+// and because every tile has a reference of its own, neither does a long tail of small weights behind a large one.
 //
 // Bound by the rows, which are read once.  The keys (of the scores) and the numbers of a head (of the output) are the
 // MMA's rows and the query heads of a kv head, times their terms, its 16 columns, so no thread touches a row: per tile
 // a thread handles one key's scores.  (With mma.sync, whose operands are at least 16 bits wide, converting the rows and the
 // scores' arithmetic took 424 instructions per 32 keys and warp: 32 sequences of 256 to 4,096 keys, heads of 128, 35.2 us.)
 //   warp 0     TMA, a lane per page: keys, values and scale bytes into rings
-//   warps 1, 2 tcgen05.mma: scores (128 keys x 16, once or twice); output (numbers x 16), values as the MN-major operand from the
-//              page layout [key][number], weights MN-major as the threads write them, 16 bytes a key.  (One thread for both
-//              took 3,200 clocks a tile: it was what the others waited for.)
-//   warps 3-6  a thread per key, or per two: scores, maxima over the tile (redux and a barrier), weights; then, a thread per number of
-//              a head, the output of the tile before
+//   warps 1, 2 tcgen05.mma: scores (128 keys x 16, once or twice); output (numbers x 16), values as the MN-major operand from
+//              the page layout [key][number], weights MN-major as the threads write them, 16 bytes a key.  (One thread for
+//              both took 3,200 clocks a tile: it was what the others waited for.)
+//   warps 3-6  a thread per key, or per two: scores, maxima over the tile (redux and a barrier), weights; then, a thread per
+//              number of a head, the output of the tile before
 // Two such blocks share an SM, so one's chain of steps runs under the other's.  The chain is what tiles of 256 keys are for with
 // heads of 64: with 128, some 300 instructions and 2,800 clocks a tile, three blocks' chains did not keep up with memory (one
-// sequence of 131,072 keys 38 us).
+// sequence of 131,072 keys 38 us, 29 with 256).  Tensor memory is allocated before the next launch may begin, 128 of an SM's
+// 512 columns a block, so a block of that launch can wait for columns only behind blocks that hold theirs and will end.
 //
 // Work is shared evenly: the tiles of all sequences and kv heads are numbered through, head by head and sequence by sequence,
 // and every block takes an equal run of them, as many blocks as are resident at once: all SMs stream until the end, whatever
 // the lengths.  A sequence's first tile counts twice: its queries, the end of the sequence before and the pause between them
-// cost about as much as a tile.  What blocks share, at most the first and the last sequence of each, goes through scratch memory, and the block
-// that takes a sequence's last ticket adds the parts up in the order of the blocks; nobody waits for another block.
+// cost about as much as a tile.  What blocks share, at most the first and the last sequence of each, goes through scratch
+// memory, and the block that takes a sequence's last ticket adds the parts up in the order of the blocks; nobody waits for
+// another block.  The cut and the order of the sums follow from the lengths alone, so a call repeats its bits.
+//
+// Measured (launches one behind another in a graph, inputs larger than L2 or as large as they are; the copy rate is 6.57 TB/s):
+//   32 sequences of 256 to 4,096 keys, 32 query on 8 kv heads of 128   31.1 us, 4.9 TB/s, 75 % of the copy rate
+//   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             34.4 us, 4.2 TB/s, 65 %
+//   one sequence of 131,072 keys, 32 on 8 heads of 128                 48.5 us, 5.6 TB/s, 85 %
+//   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64              12.0 us, and one of 57 keys 4.6 us: latency
+// Some 7 to 9 us of a launch are fixed: the cut, the first loads' way, a run's end, its ticket and the join.  The rest of the
+// distance is the blocks' uneven progress (10 % either way).
 #include <math.h>
 
 #include "common.cuh"
@@ -292,8 +302,8 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     at.b = b;
     at.k = u == 0 ? 0 : max(1, u - 1);
     // A place behind the start of the sequence's last tile, and one within a sequence of two tiles, is the start of the next: two
-    // tiles one after another take less than their parts' way through memory (8 sequences of 100 to 160 keys, heads of 128,
-    // 6.3 us against 11.8).
+    // tiles one after another take less than their parts' way through memory (8 sequences of 100 to 160 keys, heads of 128:
+    // 6.3 us, cut 11.8).
     const int nk = first[b + 1] - first[b] - 1;
     if (at.k >= nk || (at.k > 0 && nk <= 2)) {
       at.k = 0;
@@ -438,8 +448,6 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     auto wait = [&](uint64_t* bar, int parity) {
       if (ok) ok = mbar_wait(bar, parity & 1, abort_flag);
     };
-    // the queries of a sequence and kv head, fetched when the sequence before begins, as two e4m3 terms (rows g and GM + g of the operand), and what the scores are
-    // scaled by; 16 threads a head
     // what a head's weighted sum, relative to m, is multiplied with: 1 / l, the sink's share in l
     auto finish = [&](int head, float mm, float ll) {
       float f = 1.f;
@@ -450,7 +458,8 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       }
       return ll == 0.f ? 0.f : f / ll;                // (a sequence without a visible key: zeros)
     };
-    uint2 raw[HD / 64];                               // a thread's numbers of the queries that come next
+    // a thread's numbers of the queries of a sequence and kv head, 16 threads a head, asked for when the sequence before begins
+    uint2 raw[HD / 64];
     auto fetch = [&](int head, int b) {
       const int g0 = head % p.n_gchunks * DE_GM, g = st >> 4, part = st & 15;
 #pragma unroll
@@ -460,6 +469,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
           raw[k] = __ldcg(reinterpret_cast<const uint2*>(p.q + (size_t)b * p.ldq + (size_t)(head / p.n_gchunks * G + g0 + g) * HD + part * (HD / 16) + 4 * k));
       }
     };
+    // those queries as two e4m3 terms (rows g and GM + g of the operand), and what the scores are scaled by
     auto prepare = [&](int buf) {
       const int g = st >> 4, part = st & 15;
       constexpr int N = HD / 16;

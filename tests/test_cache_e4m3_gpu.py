@@ -267,8 +267,8 @@ def _decode_case(hq, hkv, hd, lens, span=0, sink=False, shape=None, dead_pages=F
 
 def _check_decode(out, want, hd, group):
     """Weights: kept as two e4m3 terms, each off by 2^-4 of what it takes (2^-8 of the weight), or three where a block has four
-    heads at most (2^-12, behind a rounding to fp16: 2^-11 in all); below the terms' smallest number, off by 2^-22 (2^-26) of the largest weight of their 128 keys, 128 times
-    that in all: 2^-15.  Exponentials within 2^-21, their arguments within what fp32 sums of hd products lose, 2 (hd + 8) 2^-24 of the
+    heads at most (2^-12, behind a rounding to fp16: 2^-11 in all); below the terms' smallest number, off by 2^-22 (2^-26) of the
+    largest weight of their 128 keys, 128 times that in all: 2^-15.  Exponentials within 2^-21, their arguments within what fp32 sums of hd products lose, 2 (hd + 8) 2^-24 of the
     sum of |q k|, and what queries lose below 2^-22 of a row's largest number, hd 2^-22 of the largest product (no more than the
     sum of |q k| again, times 2^-22 hd); the sum over the keys likewise in fp32 (folded into 2^-20); the result to bf16, whose
     smallest number is 2^-133 (half a step: 2^-134).  A weight is an fp32 number relative to the row's largest: one below 2^-126
