@@ -39,13 +39,18 @@
 // the lengths.  A sequence's first tile counts twice: its queries, the end of the sequence before and the pause between them
 // cost about as much as a tile.  What blocks share, at most the first and the last sequence of each, goes through scratch
 // memory, and the block that takes a sequence's last ticket adds the parts up in the order of the blocks; nobody waits for
-// another block.  The cut and the order of the sums follow from the lengths alone, so a call repeats its bits.
+// another block.  With few sequences every block takes tiles of one sequence alone, so that it has one end to come to, not
+// two: where a block for each of these parts is there and the longest is no more than two tiles above an equal share (with
+// none above, 16 sequences of 64 to 2,048 keys, 24 on 8 heads of 128, 16.6 us, with two 13.4; five are no faster), sequences of
+// up to three tiles whole (8 of 300 to 1,700 keys, 32 on 8 heads of 64, 9.9 us; up to four 10.7, six 11.8).  Against equal
+// runs: these 8 sequences 9.1 us for 12.3, the 16 12.7 for 16.2.
+// The cut and the order of the sums follow from the lengths alone, so a call repeats its bits.
 //
 // Measured (launches one behind another in a graph, inputs larger than L2 or as large as they are; the copy rate is 6.57 TB/s):
 //   32 sequences of 256 to 4,096 keys, 32 query on 8 kv heads of 128   31.1 us, 4.9 TB/s, 75 % of the copy rate
 //   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             34.4 us, 4.2 TB/s, 65 %
 //   one sequence of 131,072 keys, 32 on 8 heads of 128                 48.5 us, 5.6 TB/s, 85 %
-//   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64              12.0 us, and one of 57 keys 4.6 us: latency
+//   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64               9.1 us, and one of 57 keys 4.4 us: latency
 // Some 7 to 9 us of a launch are fixed: the cut, the first loads' way, a run's end, its ticket and the join.  The rest of the
 // distance is the blocks' uneven progress (10 % either way).
 #include <math.h>
@@ -64,6 +69,8 @@ constexpr int DE_SOFT = 128;          // of them, warps 3-6
 template <int HD> constexpr int de_halves = HD <= 64 ? 2 : 1;
 constexpr int DE_GM = 8;              // query heads of a kv head per block at most
 constexpr int DE_MIN_RUN = 2;         // a block's least run (so that none lies within one tile)
+constexpr int DE_WHOLE = 3;           // tiles of a sequence that is not cut where every block has one sequence's tiles alone
+constexpr int DE_SLACK = 2;           // tiles that such a block may have beyond an equal share
 constexpr int DE_MAX_B = 1024;        // sequences of a launch (their first tiles, positions and slots lie in shared memory)
 constexpr int DE_BARS = 40;           // room for barriers
 constexpr int DE_SC = 3;              // tiles whose scale bytes are on their way or in use
@@ -85,6 +92,8 @@ struct DecE8 {
   const int* token_pos;    // [B] position of the new token (its row is in the cache); -1: nothing to see, zeros come out
   __nv_bfloat16* out;      // [B][ldo]
   int ldo, B, Hq, Hkv, n_gchunks, span;
+  int room;                // blocks for each kv head (and chunk of its query heads), at most
+  float one_by_room;
   float scale_log2e;
   const float* sink;       // [Hq] or null: exp(sink) joins the denominator
   float* part_acc;         // [blocks][2][GM][HD]  O relative to m
@@ -215,6 +224,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
   volatile int* abort_flag = sums + 9;
   int* last_s = sums + 10;                            // [2] this block has a shared sequence's last ticket
   int* shared_s = sums + 16;                          // [2][4] head, sequence, first block, parts of the sequences it shares
+  int* plan_s = sums + 24;                            // [2] first block and parts of this block's sequence (0: equal runs)
   int* first = (int*)(smem + de_off_seq<HD>);         // [B + 1] first tile of each sequence
   const int B = p.B, G = p.Hq / p.Hkv, heads = p.Hkv * p.n_gchunks;
   int* pos_s = first + B + 1;                         // [B] last visible position
@@ -296,6 +306,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     at.head = (int)(narrow ? (unsigned)x / (unsigned)P : x / P);
     const int y = (int)(x - (long long)at.head * P);
     int b = -1;                                       // the last sequence whose first count is no more than y
+#pragma unroll 1
     for (int i = lane; i < B; i += 32) b += first[i] <= y;
     b = __reduce_add_sync(0xffffffffu, b + 1) - 1;
     const int u = y - first[b];
@@ -315,11 +326,67 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     enter(at);
     return at;
   };
-  int n_tiles = 0;
+  int n_tiles = 0, own_parts = 0, own_first = 0;
   DecPlace start = {0, 0, 0, 1, 1};
-  if (blockIdx.x < nb) {
-    start = place(start_of(blockIdx.x));
-    const DecPlace end = place(start_of(blockIdx.x + 1));
+  // Few sequences: every block takes tiles of one alone, about r at most, with r the least number that leaves a block for each
+  // part.  (Every block counts the same, so r's quotients may be off by a rounding.  This runs before every launch's first load:
+  // with divisions of whole numbers and unrolled loops it took a microsecond more.)
+  if (B <= p.room) {
+    const int least = (int)((P - B) * p.one_by_room) + 1;
+    int r = least, limit = max(DE_WHOLE, least + DE_SLACK), all;
+    float one_by_r;
+    auto parts_of = [&](int i) {
+      const int n = i < B ? first[i + 1] - first[i] - 1 : 0;
+      return n <= DE_WHOLE ? min(n, 1) : min((int)((n - 1) * one_by_r) + 1, n);
+    };
+    for (; r <= limit; ++r) {
+      one_by_r = __fdividef(1.f, r);
+      all = 0;
+#pragma unroll 1
+      for (int i = lane; i < B; i += 32) all += parts_of(i);
+      all = __reduce_add_sync(0xffffffffu, all);
+      if (all <= p.room) break;
+    }
+    if (r <= limit) {
+      own_parts = -1;                                 // (a block without a part)
+      if ((int)blockIdx.x < heads * all) {
+        start.head = (int)__fdividef(blockIdx.x + 0.5f, all);
+        int y = (int)blockIdx.x - start.head * all;
+#pragma unroll 1
+        for (int i0 = 0; i0 < B; i0 += 32) {
+          const int mine = parts_of(i0 + lane);
+          int upto = mine;
+#pragma unroll 1
+          for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += up;
+          }
+          const unsigned behind = __ballot_sync(0xffffffffu, upto > y);
+          if (behind) {
+            const int at = __ffs(behind) - 1;
+            own_parts = __shfl_sync(0xffffffffu, mine, at);
+            const int j = y - __shfl_sync(0xffffffffu, upto - mine, at);
+            own_first = (int)blockIdx.x - j;
+            start.b = i0 + at;
+            start.nk = first[start.b + 1] - first[start.b] - 1;
+            const int each = (int)((unsigned)start.nk / (unsigned)own_parts), more = start.nk - each * own_parts;
+            start.k = j * each + min(j, more);
+            n_tiles = each + (j < more ? 1 : 0);      // (the first `more` parts have one more)
+            enter(start);
+            break;
+          }
+          y -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+      }
+    }
+  }
+  if (own_parts == 0 && blockIdx.x < nb) {
+    DecPlace end;
+#pragma unroll 1
+    for (int e = 0; e < 2; ++e) {
+      end = place(start_of(blockIdx.x + e));
+      if (e == 0) start = end;
+    }
     // tiles up to a place: those of the heads and sequences before it, and its k
     n_tiles = (end.head - start.head) * (P - B) + (first[end.b] - end.b + end.k) - (first[start.b] - start.b + start.k);
   }
@@ -520,6 +587,10 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       prepare(0);
     }
     if (st < 2) shared_s[4 * st + 3] = 0;
+    if (st == 0) {
+      plan_s[0] = own_first;
+      plan_s[1] = own_parts;
+    }
     soft_sync();
     int seg = 0, k_first = 0, before[2] = {0, 0};
     bool fresh = true;
@@ -733,11 +804,11 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
             before[0] = side == 0 ? was : before[0];
             before[1] = side == 1 ? was : before[1];
             const long long unit = (long long)at.head * P + first[at.b];
-            const int i0 = block_of(unit);
+            const int i0 = plan_s[1] ? plan_s[0] : block_of(unit);
             shared_s[4 * side] = at.head;
             shared_s[4 * side + 1] = at.b;
             shared_s[4 * side + 2] = i0;
-            shared_s[4 * side + 3] = block_of(unit + (at.nk == 1 ? 0 : at.nk)) - i0 + 1;
+            shared_s[4 * side + 3] = plan_s[1] ? plan_s[1] : block_of(unit + (at.nk == 1 ? 0 : at.nk)) - i0 + 1;
           }
         }
         ++seg;
@@ -910,6 +981,8 @@ DLGO_EXPORT int dlgo_attention_decode_e4m3(const void* q, int B, int ldq, const 
   p.ldo = ldo; p.Hq = Hq; p.Hkv = Hkv;
   p.n_gchunks = (G + DE_GM - 1) / DE_GM;
   p.span = span; p.scale_log2e = scale * 1.4426950408889634f; p.sink = sink;
+  p.room = decode_e8_blocks() / (Hkv * p.n_gchunks);
+  p.one_by_room = p.room > 0 ? 1.f / p.room : 0.f;
   p.part_acc = scratch;
   p.part_ml = scratch + (size_t)decode_e8_blocks() * 2 * gm * hd;
   for (int b0 = 0; b0 < B; b0 += DE_MAX_B) {       // (one launch as a rule; they run one after another and share the scratch)

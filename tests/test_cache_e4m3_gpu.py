@@ -578,3 +578,15 @@ def test_keywords_alone_and_an_output_in_the_queries_place():
     _check_decode(K().attention_decode_e4m3(**dict(zip(names, args)), **more), want, hd, hq // hkv)
     with pytest.raises(K().KernelError, match="another tensor"):
         K().attention_decode_e4m3(*args, **more, out=args[0])
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 2, 64), (8, 1, 128), (32, 8, 128), (74, 37, 64)])
+@pytest.mark.parametrize("lens", [[700], [513, 1], [5000, 300, 260, 1], [129] * 4 + [20000], [900 + 37 * i for i in range(9)],
+                                  [200 * (1 + i % 7) for i in range(37)], [100] * 74 + [1500], [40] * 148, [64 * i + 1 for i in range(40)]])
+def test_decode_where_blocks_keep_to_one_sequence_and_where_they_do_not(hq, hkv, hd, lens):
+    """Numbers of sequences and heads about where a block for each part just is or is not there; sequences whole and cut."""
+    args, more, want = _decode_case(hq, hkv, hd, lens)
+    tickets = torch.zeros(len(lens) * hkv, dtype=torch.int32, device=DEV)
+    out = K().attention_decode_e4m3(*args, **more, tickets=tickets)
+    _check_decode(out, want, hd, hq // hkv)
+    assert (tickets == 0).all() and torch.equal(out, K().attention_decode_e4m3(*args, **more, tickets=tickets))
