@@ -49,8 +49,8 @@
 // Measured (launches one behind another in a graph, inputs larger than L2 or as large as they are; the copy rate is 6.57 TB/s):
 //   32 sequences of 256 to 4,096 keys, 32 query on 8 kv heads of 128   31.1 us, 4.9 TB/s, 75 % of the copy rate
 //   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             34.4 us, 4.2 TB/s, 65 %
-//   one sequence of 131,072 keys, 32 on 8 heads of 128                 48.5 us, 5.6 TB/s, 85 %
-//   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64               9.1 us, and one of 57 keys 4.4 us: latency
+//   one sequence of 131,072 keys, 32 on 8 heads of 128                 46.5 us, 5.8 TB/s, 89 %
+//   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64               8.9 us, and one of 57 keys 4.5 us: latency
 // Some 7 to 9 us of a launch are fixed: the cut, the first loads' way, a run's end, its ticket and the join.  The rest of the
 // distance is the blocks' uneven progress (10 % either way).
 #include <math.h>
@@ -143,6 +143,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Operand descriptors.  Rows of HD bytes as TMA leaves them: 128-byte swizzle for heads of 128, 64-byte swizzle for heads of 64;
 // eight rows are HD * 8 bytes, as the K-major operand (keys, queries) and as the MN-major one (values).
 template <int HD> __device__ __forceinline__ uint64_t desc_rows(uint32_t addr) {
@@ -177,7 +182,8 @@ struct DecPlace {
 // Shared memory: rings of keys and of values, two buffers of queries and of weights, scale bytes, barriers, ... , sequences
 template <int HD> constexpr int de_off_q = (DE_KST + DE_VST) * de_halves<HD> * 128 * HD;
 template <int HD> constexpr int de_off_p = de_off_q<HD> + 2 * 16 * HD;
-template <int HD> constexpr int de_off_sc = de_off_p<HD> + 2 * de_halves<HD> * 2048;
+// (6 KB to spare with heads of 128: where 8 kv heads share 296 blocks, the 37 parts of a sequence are joined in one go)
+template <int HD> constexpr int de_off_sc = de_off_p<HD> + 2 * de_halves<HD> * 2048 + (HD == 128 ? 6144 : 0);
 template <int HD> constexpr int de_off_bars = de_off_sc<HD> + DE_SC * de_halves<HD> * 256;
 template <int HD> constexpr int de_off_red = de_off_bars<HD> + DE_BARS * 8;             // [2][4][GM] floats
 template <int HD> constexpr int de_off_misc = de_off_red<HD> + 2 * 4 * DE_GM * 4;    // row scales [2][GM], maxima and sums [GM][4], words
@@ -190,7 +196,9 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
   constexpr int TERMS = GM <= 4 ? 3 : 2;
   constexpr int H = de_halves<HD>, KST = DE_KST, VST = DE_VST, STAGE = H * 128 * HD, PAGE_BYTES = E8_PAGE * HD;
   constexpr uint32_t TMEM_COLS = 128, O_COL = 64;     // scores of two tiles in columns 0 to 63, outputs in 64 and 80
-  constexpr int H4 = HD / 4, JN = 6;
+  constexpr int H4 = HD / 4;
+  // joining parts: columns of four numbers at a time, bytes of them and their maxima and sums, parts that shared memory holds
+  constexpr int JC = GM * H4 < DE_SOFT ? GM * H4 : DE_SOFT, JREC = JC * 16 + GM * 8, JN = de_off_sc<HD> / JREC;
   // the swizzled tiles want 1024-byte alignment (checked: a misaligned start ends the kernel with the error word set)
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
@@ -829,52 +837,55 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       if (!last_s[side]) continue;                    // (block-uniform)
       const int head = shared_s[4 * side], b = shared_s[4 * side + 1], i0 = shared_s[4 * side + 2], parts = shared_s[4 * side + 3];
       const int first_head = head / p.n_gchunks * G + head % p.n_gchunks * DE_GM;
-      // a thread per four numbers, or 2, 4, 8 threads that share the parts; several parts in flight each
+      // The parts of 128 columns of four numbers at a time (or of all), by way of shared memory, which nothing else uses any more:
+      // all of them on their way at once, a thread then adds up one column's.  37 parts take 2.7 us.  (In registers, six in
+      // flight, 4.6; with more in flight longer, by the unrolled instructions, which a launch has to fetch anew.)
       const int cols = min(GM, G - head % p.n_gchunks * DE_GM) * H4;
-      int tpc = 1;
-      while (tpc < 8 && cols * tpc * 2 <= DE_SOFT) tpc *= 2;
-      for (int c0 = 0; c0 < cols; c0 += DE_SOFT / tpc) {
-        const int col = c0 + st / tpc;
-        const int g = min(col, cols - 1) / H4, d = min(col, cols - 1) % H4 * 4;
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += JC) {
+        const int g = min(c0 + st, cols - 1) / H4;
         float mm = -1e30f, ll = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = st % tpc; k0 < parts; k0 += JN * tpc) {
-          float2 ml[JN];
-          float4 v[JN];
-#pragma unroll
-          for (int j = 0; j < JN; ++j) {
-            const int k = k0 + j * tpc;
-            const size_t x = ((size_t)(i0 + min(k, parts - 1)) * 2 + (k == 0 ? 1 : 0)) * GM + g;
-            ml[j] = k < parts ? __ldcg(reinterpret_cast<const float2*>(p.part_ml) + x) : make_float2(-1e30f, 0.f);
-            v[j] = k < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_acc + x * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+        for (int k0 = 0; k0 < parts; k0 += JN) {
+          const int n = min(JN, parts - k0);
+          soft_sync();                                // (those before are read)
+          const float* src = p.part_acc + (size_t)(i0 + k0 + st / JC) * 2 * GM * HD + (c0 + st % JC) * 4;
+          const uint32_t dst = smem_u32(smem + st % JC * 16);
+#pragma unroll 2
+          for (int k = st / JC; k < n; k += DE_SOFT / JC) {
+            copy16(dst + k * JREC, src + (k0 + k == 0 ? GM * HD : 0));      // (a sequence's first part is the second of its block)
+            src += DE_SOFT / JC * 2 * GM * HD;
           }
+#pragma unroll 1
+          for (int e = st; e < n * (GM / 2); e += DE_SOFT) {
+            const int k = e / (GM / 2);
+            const size_t x = (size_t)(i0 + k0 + k) * 2 + (k0 + k == 0 ? 1 : 0);
+            copy16(smem_u32(smem + JC * 16 + e % (GM / 2) * 16) + k * JREC, p.part_ml + x * GM * 2 + e % (GM / 2) * 4);
+          }
+          copies_wait();
+          soft_sync();
+          const uint8_t* ml = smem + JC * 16 + g * 8;
           float top = mm;
-#pragma unroll
-          for (int j = 0; j < JN; ++j) top = fmaxf(top, ml[j].x);
+#pragma unroll 4
+          for (int k = 0; k < n; ++k) top = fmaxf(top, *reinterpret_cast<const float*>(ml + k * JREC));
           const float keep = exp2_fast(mm - top);
           mm = top;
           ll *= keep; a.x *= keep; a.y *= keep; a.z *= keep; a.w *= keep;
-#pragma unroll
-          for (int j = 0; j < JN; ++j) {
-            const float w = exp2_fast(ml[j].x - top);
-            ll = fmaf(w, ml[j].y, ll);
-            a.x = fmaf(w, v[j].x, a.x); a.y = fmaf(w, v[j].y, a.y);
-            a.z = fmaf(w, v[j].z, a.z); a.w = fmaf(w, v[j].w, a.w);
+          const uint8_t* col = smem + st % JC * 16;
+#pragma unroll 4
+          for (int k = 0; k < n; ++k) {
+            const float2 x = *reinterpret_cast<const float2*>(ml + k * JREC);
+            const float4 v = *reinterpret_cast<const float4*>(col + k * JREC);
+            const float w = exp2_fast(x.x - top);
+            ll = fmaf(w, x.y, ll);
+            a.x = fmaf(w, v.x, a.x); a.y = fmaf(w, v.y, a.y);
+            a.z = fmaf(w, v.z, a.z); a.w = fmaf(w, v.w, a.w);
           }
         }
-        for (int x = tpc >> 1; x > 0; x >>= 1) {
-          const float m2 = __shfl_xor_sync(0xffffffffu, mm, x), top = fmaxf(mm, m2);
-          const float k1 = exp2_fast(mm - top), k2 = exp2_fast(m2 - top);
-          mm = top;
-          ll = ll * k1 + __shfl_xor_sync(0xffffffffu, ll, x) * k2;
-          a.x = a.x * k1 + __shfl_xor_sync(0xffffffffu, a.x, x) * k2;
-          a.y = a.y * k1 + __shfl_xor_sync(0xffffffffu, a.y, x) * k2;
-          a.z = a.z * k1 + __shfl_xor_sync(0xffffffffu, a.z, x) * k2;
-          a.w = a.w * k1 + __shfl_xor_sync(0xffffffffu, a.w, x) * k2;
-        }
-        if (col < cols && st % tpc == 0) {
+        if (st < JC && c0 + st < cols) {
           const float f = finish(first_head + g, mm, ll);
-          *reinterpret_cast<uint2*>(p.out + (size_t)b * p.ldo + (size_t)(first_head + g) * HD + d) =
+          *reinterpret_cast<uint2*>(p.out + (size_t)b * p.ldo + (size_t)first_head * HD + (c0 + st) * 4) =
               make_uint2(bf16_word(a.x * f, a.y * f), bf16_word(a.z * f, a.w * f));
         }
       }

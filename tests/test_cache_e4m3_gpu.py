@@ -590,3 +590,11 @@ def test_decode_where_blocks_keep_to_one_sequence_and_where_they_do_not(hq, hkv,
     out = K().attention_decode_e4m3(*args, **more, tickets=tickets)
     _check_decode(out, want, hd, hq // hkv)
     assert (tickets == 0).all() and torch.equal(out, K().attention_decode_e4m3(*args, **more, tickets=tickets))
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 1, 128), (8, 1, 64), (3, 1, 64), (16, 1, 128), (2, 2, 128)])
+def test_decode_joins_more_parts_than_shared_memory_holds(hq, hkv, hd):
+    """One long sequence, its blocks' parts joined in several goes; and a second behind it, of a few parts."""
+    for lens in ([60000], [40000, 1500]):
+        args, more, want = _decode_case(hq, hkv, hd, lens)
+        _check_decode(K().attention_decode_e4m3(*args, **more), want, hd, hq // hkv)
