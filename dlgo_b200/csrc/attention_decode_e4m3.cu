@@ -47,12 +47,13 @@
 // The cut and the order of the sums follow from the lengths alone, so a call repeats its bits.
 //
 // Measured (launches one behind another in a graph, inputs larger than L2 or as large as they are; the copy rate is 6.57 TB/s):
-//   32 sequences of 256 to 4,096 keys, 32 query on 8 kv heads of 128   31.1 us, 4.9 TB/s, 75 % of the copy rate
-//   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             34.4 us, 4.2 TB/s, 65 %
-//   one sequence of 131,072 keys, 32 on 8 heads of 128                 46.5 us, 5.8 TB/s, 89 %
-//   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64               8.9 us, and one of 57 keys 4.5 us: latency
+//   32 sequences of 256 to 4,096 keys, 32 query on 8 kv heads of 128   30.8 us, 5.0 TB/s, 76 % of the copy rate
+//   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             33.3 us, 4.4 TB/s, 67 %
+//   one sequence of 131,072 keys, 32 on 8 heads of 128                 46.1 us, 5.9 TB/s, 89 %
+//   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64               8.8 us, and one of 57 keys 4.2 us: latency
 // Some 7 to 9 us of a launch are fixed: the cut, the first loads' way, a run's end, its ticket and the join.  The rest of the
-// distance is the blocks' uneven progress (10 % either way).
+// distance is the blocks' uneven progress (10 % either way).  What a launch runs once it fetches anew, so the code is kept short
+// where it runs once a sequence: a lane per head at its end, one copy of what takes an output in (34.5 to 33.3 us, 64 sequences).
 #include <math.h>
 
 #include "common.cuh"
@@ -531,7 +532,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
         f = exp2_fast(mm - top);
         ll = fmaf(ll, f, exp2_fast(sk - top));
       }
-      return ll == 0.f ? 0.f : f / ll;                // (a sequence without a visible key: zeros)
+      return ll == 0.f ? 0.f : __fdividef(f, ll);                // (a sequence without a visible key: zeros)
     };
     // a thread's numbers of the queries of a sequence and kv head, 16 threads a head, asked for when the sequence before begins
     uint2 raw[HD / 64];
@@ -602,11 +603,11 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     soft_sync();
     int seg = 0, k_first = 0, before[2] = {0, 0};
     bool fresh = true;
-    float m[GM], l[GM], N[GM], n_t[GM], o[GM], fs[GM];
+    float m[GM], l[GM], N[GM], n_t[GM], n_new[GM], o[GM], fs[GM];
     int g0 = 0, GC = 0, head0 = 0, first_key = 0, last_key = 0;       // of the sequence
     int key = 0;                                      // this thread's first; a second is 128 behind it
-    // the output of tile `it`, whose reference is n_t, into o
-    auto gather = [&](int it) {
+    // the output of tile `it` (the newest, whose reference is n_new, or the one before it: n_t) into o
+    auto gather = [&](int it, bool newest) {
       wait(&o_full[it & 1], it >> 1);
       __syncwarp();
       tc_fence_after_sync();
@@ -620,8 +621,8 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       for (int g = 0; g < GM; ++g) {
         float x = fmaf(t[GM + g], 0.0625f, t[g]);
         if (TERMS == 3) x = fmaf(t[(TERMS - 1) * GM + g], 0.00390625f, x);
-        const float top = fmaxf(N[g], n_t[g]);
-        o[g] = fmaf(o[g], exp2_fast(N[g] - top), x * exp2_fast(n_t[g] - top));
+        const float n = newest ? n_new[g] : n_t[g], top = fmaxf(N[g], n);
+        o[g] = fmaf(o[g], exp2_fast(N[g] - top), x * exp2_fast(n - top));
         N[g] = top;
       }
     };
@@ -698,7 +699,6 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
         m[g] = m_new;
       }
       soft_sync();
-      float n_new[GM];
 #pragma unroll
       for (int g = 0; g < GM; g += 4) {
         float4 x = *reinterpret_cast<const float4*>(red + g);
@@ -749,13 +749,13 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[it & 1]);
-      if (!fresh) gather(it - 1);
+#pragma unroll 1
+      for (int t = fresh ? it : it - 1; t < it + ends; ++t) gather(t, t == it);
 #pragma unroll
       for (int g = 0; g < GM; ++g) n_t[g] = n_new[g];
       fresh = ends;
       key += 128 * H;
       if (ends) {
-        gather(it);
         // the sequence's result, or this block's part of it
         const bool whole = k_first == 0 && at.k + 1 == at.nk;
         // the threads' sums: to the warp's maximum, then half of the heads handed over at every step (a lane ends with one
@@ -783,22 +783,23 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
         soft_sync();
         const int side = k_first == 0 ? 1 : 0;        // (a block shares two sequences at most: one that began before, one after)
         const size_t part0 = ((size_t)blockIdx.x * 2 + side) * GM;
+        // lane g: head g's maximum and sum over the warps, and its last factor
+        const int gl = lane % GM;
+        const float2 w0 = ml_s[gl * 4], w1 = ml_s[gl * 4 + 1], w2 = ml_s[gl * 4 + 2], w3 = ml_s[gl * 4 + 3];
+        const float mm = fmaxf(fmaxf(w0.x, w1.x), fmaxf(w2.x, w3.x));
+        const float ll = fmaf(w0.y, exp2_fast(w0.x - mm), w1.y * exp2_fast(w1.x - mm)) +
+                         fmaf(w2.y, exp2_fast(w2.x - mm), w3.y * exp2_fast(w3.x - mm));
+        float f = 1.f;
+        if (whole) f = finish(head0 + min(gl, GC - 1), mm, ll);
+        else if (st < GM) *reinterpret_cast<float2*>(p.part_ml + (part0 + gl) * 2) = make_float2(mm, ll);
 #pragma unroll
         for (int g = 0; g < GM; ++g) {
-          if (g >= GC) continue;
-          const float2 w0 = ml_s[g * 4], w1 = ml_s[g * 4 + 1], w2 = ml_s[g * 4 + 2], w3 = ml_s[g * 4 + 3];
-          const float mm = fmaxf(fmaxf(w0.x, w1.x), fmaxf(w2.x, w3.x));
-          const float ll = fmaf(w0.y, exp2_fast(w0.x - mm), w1.y * exp2_fast(w1.x - mm)) +
-                           fmaf(w2.y, exp2_fast(w2.x - mm), w3.y * exp2_fast(w3.x - mm));
           // relative to m (in two steps: the values' powers may be far from the weights')
-          const float half = exp2_fast(0.5f * (N[g] - 8.f - mm)), x = o[g] * half * half;
-          if (whole) {
-            const float f = finish(head0 + g, mm, ll);
-            if (has_dim) p.out[(size_t)at.b * p.ldo + (size_t)(head0 + g) * HD + dim] = __float2bfloat16_rn(x * f);
-          } else {
-            if (has_dim) p.part_acc[(part0 + g) * HD + dim] = x;
-            if (st == 0) *reinterpret_cast<float2*>(p.part_ml + (part0 + g) * 2) = make_float2(mm, ll);
-          }
+          const float half = exp2_fast(0.5f * (N[g] - 8.f - __shfl_sync(0xffffffffu, mm, g)));
+          const float x = o[g] * half * half * __shfl_sync(0xffffffffu, f, g);
+          if (g >= GC || !has_dim) continue;
+          if (whole) p.out[(size_t)at.b * p.ldo + (size_t)(head0 + g) * HD + dim] = __float2bfloat16_rn(x);
+          else p.part_acc[(part0 + g) * HD + dim] = x;
         }
         if (!whole) {
           // This block's part is written; its ticket now, and whether that is the last when the block's run is over.
