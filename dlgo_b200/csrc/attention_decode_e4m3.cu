@@ -1011,6 +1011,9 @@ DLGO_EXPORT int dlgo_attention_decode_e4m3(const void* q, int B, int ldq, const 
   return DLGO_OK;
 }
 
+// The same, called with a record (e4m3.cuh).
+DLGO_EXPORT int dlgo_attention_decode_e4m3_record(const long long* r) { return call_record(dlgo_attention_decode_e4m3, r); }
+
 // 1 if a bounded wait ran out since the last call (clears the word).
 DLGO_EXPORT int dlgo_attention_decode_e4m3_error() {
   int v = 0, zero = 0;

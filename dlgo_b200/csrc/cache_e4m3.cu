@@ -360,6 +360,10 @@ DLGO_EXPORT int dlgo_read_e4m3(const void* kpages, const void* vpages, const voi
   return launch_status();
 }
 
+// Both, called with a record (e4m3.cuh).
+DLGO_EXPORT int dlgo_write_e4m3_record(const long long* r) { return call_record(dlgo_write_e4m3, r); }
+DLGO_EXPORT int dlgo_read_e4m3_record(const long long* r) { return call_record(dlgo_read_e4m3, r); }
+
 // 1 if a write was skipped since the last call because its position had no page (clears the word).
 DLGO_EXPORT int dlgo_cache_e4m3_error() {
   int v = 0, zero = 0;
