@@ -22,7 +22,7 @@ struct WriteE8 {
   const int* token_seq;
   const int* seq_slot;
   const int* page_table;     // [slots][max_pages]
-  int n_slots, max_pages, n_pages, n_positions;
+  int n_seqs, n_slots, max_pages, n_pages, n_positions;
   uint8_t* kpages;           // [n_pages][Hkv][64][hd]
   uint8_t* vpages;
   uint8_t* kscales;          // [n_pages][Hkv][64]
@@ -37,7 +37,7 @@ __device__ __forceinline__ long long e8_row(const WriteE8& p, int t, int& pos, b
   const bool in_tables = pos >= 0 && (p.rot == 0 || pos < p.n_positions);
   int page = -1;
   if (in_tables && p.write_cache) {
-    const int slot = p.seq_slot[p.token_seq[t]], idx = pos / E8_PAGE;
+    const int seq = p.token_seq[t], slot = seq >= 0 && seq < p.n_seqs ? p.seq_slot[seq] : -1, idx = pos / E8_PAGE;
     if (slot >= 0 && slot < p.n_slots && idx < p.max_pages) page = p.page_table[(size_t)slot * p.max_pages + idx];
   }
   const bool bad = !in_tables || (p.write_cache && (page < 0 || page >= p.n_pages));
@@ -319,8 +319,8 @@ int launch_write(const WriteE8& p, cudaStream_t stream) {
 // q[T, Hq * hd] bf16; keys (rotated) and values into the 8-bit pages of those positions, unless write_cache is 0.  clear
 // (fp32 only): zeros are left where qkv was read.
 DLGO_EXPORT int dlgo_write_e4m3(void* qkv, int dtype, int T, int ld, const float* cos_t, const float* sin_t, int n_positions,
-                                const int* token_pos, const int* token_seq, const int* seq_slot, const int* page_table, int n_slots, int max_pages,
-                                void* kpages, void* vpages, void* kscales, void* vscales, int n_pages, void* q, int Hq, int Hkv, int hd,
+                                const int* token_pos, const int* token_seq, const int* seq_slot, int n_seqs, const int* page_table,
+                                int n_slots, int max_pages, void* kpages, void* vpages, void* kscales, void* vscales, int n_pages, void* q, int Hq, int Hkv, int hd,
                                 int rot, int interleaved, int write_cache, int clear, cudaStream_t stream) {
   if (T <= 0) return DLGO_OK;
   if (Hq <= 0 || Hkv <= 0 || (hd != 64 && hd != 128) || rot < 0 || rot > hd || rot % 2 || (rot > 0 && n_positions <= 0) ||
@@ -334,7 +334,7 @@ DLGO_EXPORT int dlgo_write_e4m3(void* qkv, int dtype, int T, int ld, const float
     return DLGO_ERR_ALIGN;
   WriteE8 p;
   p.qkv = qkv; p.ld = ld; p.cos_t = cos_t; p.sin_t = sin_t; p.token_pos = token_pos; p.token_seq = token_seq; p.seq_slot = seq_slot;
-  p.page_table = page_table; p.n_slots = n_slots; p.max_pages = max_pages; p.n_pages = n_pages;
+  p.n_seqs = n_seqs; p.page_table = page_table; p.n_slots = n_slots; p.max_pages = max_pages; p.n_pages = n_pages;
   p.n_positions = n_positions;
   p.kpages = (uint8_t*)kpages; p.vpages = (uint8_t*)vpages; p.kscales = (uint8_t*)kscales; p.vscales = (uint8_t*)vscales;
   p.q = (__nv_bfloat16*)q; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.rot = rot; p.interleaved = interleaved; p.write_cache = write_cache;

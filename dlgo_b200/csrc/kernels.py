@@ -1534,7 +1534,7 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, to
     bfloat16.  ``cos`` / ``sin`` [positions, rotary_dim / 2] fp32: the first ``rotary_dim`` numbers of a head are rotated (0: none;
     the tables are then not read), in pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1).  ``write_cache`` False:
     queries only (a layer that reads another's cache).  ``clear`` (fp32): zeros are left where ``qkv`` was read.  A position
-    without a page is not written (:func:`check_device_errors` reports it).  The tokens' positions are distinct within a
+    without a page, or of a sequence that ``seq_slot`` does not have, is not written (:func:`check_device_errors` reports it).  The tokens' positions are distinct within a
     sequence."""
     what = "rope_append_e4m3"
     if num_heads <= 0 or num_kv_heads <= 0:
@@ -1558,10 +1558,10 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, to
                ("page_table", page_table, _I32), ("cos", cos, _F32T), ("sin", sin, _F32T), ("token_pos", token_pos, _I32),
                ("token_seq", token_seq, _I32), ("seq_slot", seq_slot, _I32))
     q = qkv.new_empty((T, num_heads * head_dim), dtype=torch.bfloat16)      # (half the host time of torch.empty)
-    st = _e4m3_entry("cache_e4m3", "dlgo_write_e4m3_record", "27q")(
+    st = _e4m3_entry("cache_e4m3", "dlgo_write_e4m3_record", "28q")(
         qkv.data_ptr(), code, T, qkv.stride(0) if T > 1 else cols, cos.data_ptr(), sin.data_ptr(), positions, token_pos.data_ptr(),
-        token_seq.data_ptr(), seq_slot.data_ptr(), page_table.data_ptr(), page_table.shape[0], page_table.shape[1], kpages.data_ptr(),
-        vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(), kpages.shape[0], q.data_ptr(), num_heads, num_kv_heads, head_dim,
+        token_seq.data_ptr(), seq_slot.data_ptr(), seq_slot.numel(), page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
+        kpages.data_ptr(), vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(), kpages.shape[0], q.data_ptr(), num_heads, num_kv_heads, head_dim,
         rotary_dim, interleaved, write_cache, clear)
     _check(st, what, 1 if T > 0 else 0)
     return q
@@ -2728,7 +2728,7 @@ class PromptStep(ctypes.Structure):
     _fields_ = [("tokens", _i), ("residual", _p), ("x", _p), ("qkv", _p), ("attn_out", _p), ("h", _p), ("cos_t", _p),
                 ("sin_t", _p), ("token_pos", _p), ("token_seq", _p), ("seq_slot", _p), ("page_table", _p),
                 ("max_pages", _i), ("tiles", _p), ("n_tiles", _i), ("bn", _i * 4), ("pair", _i * 4), ("fuse_rope", _i),
-                ("form", _i * 4), ("splits", _i * 4), ("qkv_sum", _p), ("q", _p), ("n_positions", _i), ("n_slots", _i), ("seen", _p),
+                ("form", _i * 4), ("splits", _i * 4), ("qkv_sum", _p), ("q", _p), ("n_positions", _i), ("n_seqs", _i), ("n_slots", _i), ("seen", _p),
                 ("n_seen", _i), ("seen_table", _p), ("seen_width", _i), ("seen_rows", _p), ("keys", _p), ("values", _p)]
 
 

@@ -32,8 +32,8 @@ typedef int (*AttentionFn)(const void* q, int T, int ldq, const void* kpages, co
                            cudaStream_t stream);
 
 typedef int (*WriteE4m3Fn)(void* qkv, int dtype, int T, int ld, const float* cos_t, const float* sin_t, int n_positions,
-                           const int* token_pos, const int* token_seq, const int* seq_slot, const int* page_table, int n_slots,
-                           int max_pages, void* kpages, void* vpages, void* kscales, void* vscales, int n_pages, void* q, int Hq, int Hkv,
+                           const int* token_pos, const int* token_seq, const int* seq_slot, int n_seqs, const int* page_table,
+                           int n_slots, int max_pages, void* kpages, void* vpages, void* kscales, void* vscales, int n_pages, void* q, int Hq, int Hkv,
                            int hd, int rot, int interleaved, int write_cache, int clear, cudaStream_t stream);
 typedef int (*ReadE4m3Fn)(const void* kpages, const void* vpages, const void* kscales, const void* vscales, int n_pages,
                           const int* page_table, int n_slots, int max_pages, const int* pages, int n, void* keys, void* values, int Hkv,
@@ -123,6 +123,7 @@ struct DlgoPromptStep {
   // attention reads them there.
   void* q;                // [tokens, heads * head_dim] bf16
   int n_positions;        // rows of cos_t and sin_t
+  int n_seqs;             // entries of seq_slot
   int n_slots;            // rows of page_table
   const int* seen;        // [n_seen][3] (slot, page of its sequence, rows)
   int n_seen;
@@ -182,7 +183,8 @@ DLGO_EXPORT int dlgo_prompt_layers(const DlgoPromptEntryPoints* fn, const DlgoPr
       void* proj = sum ? (void*)p->qkv_sum : p->qkv;
       DLGO_STEP(product(0, p->x, L.w_qkv, n_cols, d, proj, n_cols, sum ? TC_ADD_F32 : TC_STORE));
       st = fn->write_e4m3(proj, sum ? DLGO_F32 : DLGO_BF16, T, n_cols, p->cos_t, p->sin_t, p->n_positions, p->token_pos, p->token_seq,
-                          p->seq_slot, p->page_table, p->n_slots, p->max_pages, L.kpages, L.vpages, L.kscales, L.vscales, L.n_pages, p->q,
+                          p->seq_slot, p->n_seqs, p->page_table, p->n_slots, p->max_pages, L.kpages, L.vpages, L.kscales, L.vscales,
+                          L.n_pages, p->q,
                           s->heads, s->kv_heads, s->head_dim, s->rotary_dim, s->interleaved, L.write_cache, sum ? 1 : 0, stream);
       if (st == DLGO_OK)
         st = fn->read_e4m3(L.kpages, L.vpages, L.kscales, L.vscales, L.n_pages, p->page_table, p->n_slots, p->max_pages, p->seen,

@@ -156,7 +156,7 @@ class PromptRun:
             seen, table, at = ctx.pages_in_sight(window, view.page_size)
             n = seen.shape[0] * hkv * view.page_size * hd
             step.q = ctx.scratch("prompt_q", T * hq * hd, torch.bfloat16).data_ptr()
-            step.n_positions, step.n_slots = (cos.shape[0] if rot else 0), view.page_table.shape[0]
+            step.n_positions, step.n_seqs, step.n_slots = (cos.shape[0] if rot else 0), ctx.seq_slot.numel(), view.page_table.shape[0]
             step.seen, step.n_seen = seen.data_ptr(), seen.shape[0]
             step.seen_table, step.seen_width, step.seen_rows = table.data_ptr(), table.shape[1], at.data_ptr()
             step.keys, step.values = (ctx.scratch(f"attention_e4m3_{name}", n, torch.bfloat16).data_ptr() for name in ("keys", "values"))

@@ -598,3 +598,20 @@ def test_decode_joins_more_parts_than_shared_memory_holds(hq, hkv, hd):
     for lens in ([60000], [40000, 1500]):
         args, more, want = _decode_case(hq, hkv, hd, lens)
         _check_decode(K().attention_decode_e4m3(*args, **more), want, hd, hq // hkv)
+
+
+@pytest.mark.parametrize("rot", [64, 32])
+def test_write_for_a_sequence_that_is_not_there_stores_nothing_and_says_so(rot):
+    hq, hkv, hd = 2, 1, 64
+    x = torch.randn(3, (hq + 2 * hkv) * hd, device=DEV)
+    cos, sin = torch.ones(4, rot // 2, device=DEV), torch.zeros(4, rot // 2, device=DEV)
+    for seq in (2, -1, 2 ** 31 - 1, -2 ** 31):
+        cache = Cache([3, 3], hkv, hd)
+        dev = cache.device()
+        q = K().rope_append_e4m3(x, cos, sin, ints([0, 1, 2]), ints([0, seq, 1]), ints(cache.slots), *dev, hq, hkv, hd, rot)
+        assert torch.equal(q, x[:, :hq * hd].to(torch.bfloat16))
+        written = torch.zeros(dev[2].shape, dtype=torch.bool)
+        written[int(cache.table[cache.slots[0], 0]), :, 0] = written[int(cache.table[cache.slots[1], 0]), :, 2] = True
+        assert torch.equal((dev[2] != 255).cpu(), written) and torch.equal((dev[0].view(torch.uint8) != 0x7F).any(-1).cpu(), written)
+        with pytest.raises(K().KernelError, match="no page"):
+            K().check_device_errors()
