@@ -48,7 +48,7 @@
 //
 // Measured (launches one behind another in a graph, inputs larger than L2 or as large as they are; the copy rate is 6.57 TB/s):
 //   32 sequences of 256 to 4,096 keys, 32 query on 8 kv heads of 128   30.8 us, 5.0 TB/s, 76 % of the copy rate
-//   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             33.3 us, 4.4 TB/s, 67 %
+//   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             32.3 us, 4.5 TB/s, 69 %
 //   one sequence of 131,072 keys, 32 on 8 heads of 128                 46.1 us, 5.9 TB/s, 89 %
 //   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64               8.8 us, and one of 57 keys 4.2 us: latency
 // Some 7 to 9 us of a launch are fixed: the cut, the first loads' way, a run's end, its ticket and the join.  The rest of the
@@ -601,7 +601,7 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
       plan_s[1] = own_parts;
     }
     soft_sync();
-    int seg = 0, k_first = 0, before[2] = {0, 0};
+    int seg = 0, k_first = 0;
     bool fresh = true;
     float m[GM], l[GM], N[GM], n_t[GM], n_new[GM], o[GM], fs[GM];
     int g0 = 0, GC = 0, head0 = 0, first_key = 0, last_key = 0;       // of the sequence
@@ -801,37 +801,32 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
           if (whole) p.out[(size_t)at.b * p.ldo + (size_t)(head0 + g) * HD + dim] = __float2bfloat16_rn(x);
           else p.part_acc[(part0 + g) * HD + dim] = x;
         }
-        if (!whole) {
-          // This block's part is written; its ticket now, and whether that is the last when the block's run is over.
-          soft_sync();
-          if (st == 0) {
-            // releases the block's part, which is behind the barrier; acquires those of the blocks before it for the
-            // other threads, behind a later one
-            int* ticket = p.tickets + (size_t)at.b * heads + at.head;
-            int was;
-            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(was) : "l"(ticket) : "memory");
-            before[0] = side == 0 ? was : before[0];
-            before[1] = side == 1 ? was : before[1];
-            const long long unit = (long long)at.head * P + first[at.b];
-            const int i0 = plan_s[1] ? plan_s[0] : block_of(unit);
-            shared_s[4 * side] = at.head;
-            shared_s[4 * side + 1] = at.b;
-            shared_s[4 * side + 2] = i0;
-            shared_s[4 * side + 3] = plan_s[1] ? plan_s[1] : block_of(unit + (at.nk == 1 ? 0 : at.nk)) - i0 + 1;
-          }
+        if (!whole && st == 0) {                      // (its ticket when the block's run is over)
+          const long long unit = (long long)at.head * P + first[at.b];
+          const int i0 = plan_s[1] ? plan_s[0] : block_of(unit);
+          shared_s[4 * side] = at.head;
+          shared_s[4 * side + 1] = at.b;
+          shared_s[4 * side + 2] = i0;
+          shared_s[4 * side + 3] = plan_s[1] ? plan_s[1] : block_of(unit + (at.nk == 1 ? 0 : at.nk)) - i0 + 1;
         }
         ++seg;
       }
       at = next;
     }
     soft_sync();
-    if (st == 0) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int parts = shared_s[4 * k + 3];
-        last_s[k] = parts > 0 && before[k] == parts - 1;
-        if (last_s[k]) p.tickets[(size_t)shared_s[4 * k + 1] * heads + shared_s[4 * k]] = 0;       // for the next launch
+    if (st < 2) {
+      // Tickets: both at once, at the run's end (in the run's middle a ticket holds the block up for 1.6 us).  Releases the
+      // block's parts, which are behind the barrier; acquires those of the blocks before it for the other threads, behind the next.
+      const int parts = shared_s[4 * st + 3];
+      bool last = false;
+      if (parts > 0) {
+        int* ticket = p.tickets + (size_t)shared_s[4 * st + 1] * heads + shared_s[4 * st];
+        int was;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(was) : "l"(ticket) : "memory");
+        last = was == parts - 1;
+        if (last) *ticket = 0;                        // for the next launch
       }
+      last_s[st] = last;
     }
     soft_sync();
     for (int side = 0; side < 2; ++side) {
