@@ -615,3 +615,14 @@ def test_write_for_a_sequence_that_is_not_there_stores_nothing_and_says_so(rot):
         assert torch.equal((dev[2] != 255).cpu(), written) and torch.equal((dev[0].view(torch.uint8) != 0x7F).any(-1).cpu(), written)
         with pytest.raises(K().KernelError, match="no page"):
             K().check_device_errors()
+
+
+def test_more_tiles_than_32_bits_count_are_refused():
+    args, more, want = _decode_case(2, 1, 64, [70])
+    table = torch.full((1, 2 ** 21), -1, dtype=torch.int32, device=DEV)
+    table[0, :2] = args[5][int(args[6][0]), :2]
+    args[5], args[6] = table, ints([0])
+    _check_decode(K().attention_decode_e4m3(*args, **more), want, 64, 2)
+    args[0], args[6], args[7] = args[0].expand(1024, -1).contiguous(), ints([0] * 1024), ints([69] * 1024)
+    with pytest.raises(K().KernelError, match="size"):
+        K().attention_decode_e4m3(*args, **more)
