@@ -626,3 +626,35 @@ def test_more_tiles_than_32_bits_count_are_refused():
     args[0], args[6], args[7] = args[0].expand(1024, -1).contiguous(), ints([0] * 1024), ints([69] * 1024)
     with pytest.raises(K().KernelError, match="size"):
         K().attention_decode_e4m3(*args, **more)
+
+
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^32 bytes of keys, written, read and attended at its last pages; more than 2^31 numbers read back."""
+    hq, hkv, hd = 16, 8, 128
+    n = 2 ** 32 // (hkv * PAGE * hd) + 8
+    kp, vp = (torch.zeros(n, hkv, PAGE, hd, dtype=torch.uint8, device=DEV) for _ in range(2))
+    ks, vs = (torch.full((n, hkv, PAGE), 127, dtype=torch.uint8, device=DEV) for _ in range(2))
+    f8 = torch.float8_e4m3fn
+    table = ints([[n - 1, n - 3], [-1, n - 2]])
+    cache = (kp.view(f8), vp.view(f8), ks, vs, table)
+    torch.manual_seed(1)
+    x = torch.randn(100, hq + 2 * hkv, hd)
+    cos, sin = torch.ones(100, hd // 2, device=DEV), torch.zeros(100, hd // 2, device=DEV)
+    q = K().rope_append_e4m3(x.reshape(100, -1).to(DEV), cos, sin, ints(range(100)), ints([0] * 100), ints([0]), *cache, hq, hkv, hd, hd)
+    K().check_device_errors()
+    rows = []
+    for h0, pages, scales in ((hq, kp, ks), (hq + hkv, vp, vs)):
+        stored, s = P.quantised(x[:, h0:h0 + hkv])
+        rows.append(stored * P.two_to(s.long() - 127).unsqueeze(-1))
+        held = P.values(pages[[n - 1, n - 3]].view(f8), scales[[n - 1, n - 3]])
+        assert torch.equal(held.transpose(1, 2).reshape(2 * PAGE, hkv, hd)[:100], rows[-1])
+        assert not pages[:n - 8].any() and not pages[n - 2].any()
+    out = K().attention_decode_e4m3(q[99:], *cache, ints([0]), ints([99]), hq, hkv, hd, hd ** -0.5)
+    _check_decode(out, [P.attend(q[99].cpu().view(hq, hd), rows[0], rows[1], hd ** -0.5, None)], hd, hq // hkv)
+    del kp, vp, pages
+    many = 2 ** 31 // (hkv * PAGE * hd) + 3
+    listed = torch.tensor([[1, 1, 0]], dtype=torch.int32).repeat(many, 1)
+    listed[-2:] = torch.tensor([[0, 1, 36], [0, 0, 64]])
+    for got, want in zip(K().read_pages_e4m3(*cache, listed.to(DEV)), rows):
+        assert torch.equal(got[-1].transpose(0, 1).double().cpu(), want[:PAGE])
+        assert torch.equal(got[-2].transpose(0, 1)[:36].double().cpu(), want[PAGE:]) and not got[-2, :, 36:].any() and not got[-3].any()
