@@ -41,15 +41,16 @@
 // memory, and the block that takes a sequence's last ticket adds the parts up in the order of the blocks; nobody waits for
 // another block.  With few sequences every block takes tiles of one sequence alone, so that it has one end to come to, not
 // two: where a block for each of these parts is there and the longest is no more than two tiles above an equal share (with
-// none above, 16 sequences of 64 to 2,048 keys, 24 on 8 heads of 128, 16.6 us, with two 13.4; five are no faster), sequences of
-// up to three tiles whole (8 of 300 to 1,700 keys, 32 on 8 heads of 64, 9.9 us; up to four 10.7, six 11.8).  Against equal
-// runs: these 8 sequences 9.1 us for 12.3, the 16 12.7 for 16.2.
+// none above, 16 sequences of 64 to 2,048 keys, 24 on 8 heads of 128, 16.6 us, with two 13.4; five are no faster).  Against
+// equal runs: these 12.7 us for 16.2, 8 of 300 to 1,700 keys 9.1 for 12.3.  Two tiles stay together either way (8 sequences of 100
+// to 160 keys, heads of 128: 6.4 us, cut 7.3); three do not (a whole layer for one sequence of 540 keys, heads of 64: 43.7 us,
+// together 45.1).
 // The cut and the order of the sums follow from the lengths alone, so a call repeats its bits.
 //
 // Measured (launches one behind another in a graph, inputs larger than L2 or as large as they are; the copy rate is 6.57 TB/s):
 //   32 sequences of 256 to 4,096 keys, 32 query on 8 kv heads of 128   30.8 us, 5.0 TB/s, 76 % of the copy rate
 //   64 sequences of 128 to 4,096 keys, 32 on 8 heads of 64             32.3 us, 4.5 TB/s, 69 %
-//   one sequence of 131,072 keys, 32 on 8 heads of 128                 46.1 us, 5.9 TB/s, 89 %
+//   one sequence of 131,072 keys, 32 on 8 heads of 128                 45.7 us, 5.9 TB/s, 90 %
 //   8 sequences of 300 to 1,700 keys, 32 on 8 heads of 64               8.8 us, and one of 57 keys 4.2 us: latency
 // Some 7 to 9 us of a launch are fixed: the cut, the first loads' way, a run's end, its ticket and the join.  The rest of the
 // distance is the blocks' uneven progress (10 % either way).  What a launch runs once it fetches anew, so the code is kept short
@@ -70,8 +71,8 @@ constexpr int DE_SOFT = 128;          // of them, warps 3-6
 template <int HD> constexpr int de_halves = HD <= 64 ? 2 : 1;
 constexpr int DE_GM = 8;              // query heads of a kv head per block at most
 constexpr int DE_MIN_RUN = 2;         // a block's least run (so that none lies within one tile)
-constexpr int DE_WHOLE = 3;           // tiles of a sequence that is not cut where every block has one sequence's tiles alone
-constexpr int DE_SLACK = 2;           // tiles that such a block may have beyond an equal share
+constexpr int DE_WHOLE = 2;           // tiles of a sequence that is not cut
+constexpr int DE_SLACK = 2;           // tiles beyond an equal share that a block may have where it has one sequence's alone
 constexpr int DE_MAX_B = 1024;        // sequences of a launch (their first tiles, positions and slots lie in shared memory)
 constexpr int DE_BARS = 40;           // room for barriers
 constexpr int DE_SC = 3;              // tiles whose scale bytes are on their way or in use
@@ -321,11 +322,9 @@ attention_decode_e4m3_kernel(const __grid_constant__ CUtensorMap map_k, const __
     const int u = y - first[b];
     at.b = b;
     at.k = u == 0 ? 0 : max(1, u - 1);
-    // A place behind the start of the sequence's last tile, and one within a sequence of two tiles, is the start of the next: two
-    // tiles one after another take less than their parts' way through memory (8 sequences of 100 to 160 keys, heads of 128:
-    // 6.3 us, cut 11.8).
+    // a place behind the start of the sequence's last tile, and one within a sequence of DE_WHOLE tiles, is the start of the next
     const int nk = first[b + 1] - first[b] - 1;
-    if (at.k >= nk || (at.k > 0 && nk <= 2)) {
+    if (at.k >= nk || (at.k > 0 && nk <= DE_WHOLE)) {
       at.k = 0;
       if (++at.b == B) {
         at.b = 0;
