@@ -1617,7 +1617,8 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
     denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives NaN.  ``out`` is
     another tensor than ``q``.  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
     ``tickets`` (a zero int32 per sequence and chunk of 8 heads of a kv head, left zero) are made here when not given; given ones
-    belong to one launch at a time."""
+    belong to one launch at a time.  Positions, slots and the page table are the step's inputs, which this kernel and the two above
+    read while the package's kernel in front of them may still run: none of those writes them."""
     what = "attention_decode_e4m3"
     if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
         raise KernelError(f"{what}: num_heads must be a multiple of num_kv_heads")
