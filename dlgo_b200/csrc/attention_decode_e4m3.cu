@@ -112,9 +112,9 @@ __device__ __forceinline__ uint32_t bf16_word(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float warp_max_redux(float x) {     // (a NaN does not count)
+__device__ __forceinline__ float warp_max_redux(float x) {     // (a NaN does not count; volatile: all lanes execute it, wherever its result is used)
   float y;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, float* v) {
