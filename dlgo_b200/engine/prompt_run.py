@@ -80,7 +80,7 @@ class PromptRun:
     def __init__(self, first: int, n: int, sig: tuple):
         self.first, self.n, self.sig = first, n, sig
         self._layers: Dict[int, tuple] = {}       # per cache (its pages are part of the descriptors)
-        self._entry: Optional[K.PromptEntryPoints] = None
+        self._entry: Dict[bool, K.PromptEntryPoints] = {}      # with those of the 8-bit cache, or without
 
     def takes(self, ctx: Any, cache: Any) -> bool:
         hd = self.sig[3]
@@ -117,8 +117,8 @@ class PromptRun:
         if residual.dtype != torch.float32 or not residual.is_contiguous() or tuple(residual.shape) != (T, d):
             raise K.KernelError("the residual stream must be contiguous float32 [tokens, hidden]")
         e4m3 = _is_e4m3(view)
-        if self._entry is None:
-            self._entry = K.prompt_entry_points(True) if e4m3 else K.prompt_entry_points()
+        if e4m3 not in self._entry:
+            self._entry[e4m3] = K.prompt_entry_points(True) if e4m3 else K.prompt_entry_points()
         layers, _keep = self._descriptors(model, cache)
         if pe_name is not None:
             pe = model.positions[pe_name]
@@ -162,7 +162,7 @@ class PromptRun:
             step.keys, step.values = (ctx.scratch(f"attention_e4m3_{name}", n, torch.bfloat16).data_ptr() for name in ("keys", "values"))
         step.fuse_rope = 1 if step.form[0] == 0 and pe_name is not None and blk.mixer.fuses_prompt_rope(ctx, view, model.positions) else 0
         shape = K.PromptShape(d, hq, hkv, hd, f, rot, 1 if inter else 0, window, view.page_size, scale)
-        K.prompt_layers(self._entry, shape, layers, step)
+        K.prompt_layers(self._entry[e4m3], shape, layers, step)
 
 
 def plan_runs(model: Any, runtime: Any) -> Dict[int, PromptRun]:
