@@ -973,6 +973,7 @@ DLGO_EXPORT int dlgo_attention_decode_e4m3(const void* q, int B, int ldq, const 
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || (hd != 64 && hd != 128) || n_pages <= 0 || n_slots <= 0 || max_pages <= 0) return DLGO_ERR_SIZE;
   if ((long long)n_pages * Hkv * E8_PAGE > 0x7fffffffLL || max_pages > 0x7fffffff / E8_PAGE) return DLGO_ERR_SIZE;
   if ((long long)max_pages * (B < DE_MAX_B ? B : DE_MAX_B) > 0x7fffffffLL) return DLGO_ERR_SIZE;       // (a launch's tiles are counted in 32 bits)
+  if (B > 1 && (ldq < 0 || ldo < Hq * hd)) return DLGO_ERR_SIZE;        // (rows of the output that meet would depend on the blocks' order)
   if ((ldq & 3) || (ldo & 3) || ((uintptr_t)q & 7) || ((uintptr_t)out & 7) || ((uintptr_t)kpages & 15) || ((uintptr_t)vpages & 15) ||
       ((uintptr_t)kscales & 15) || ((uintptr_t)vscales & 15) || ((uintptr_t)scratch & 15) || scratch == nullptr || tickets == nullptr)
     return DLGO_ERR_ALIGN;

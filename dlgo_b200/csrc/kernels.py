@@ -1497,6 +1497,24 @@ def _need_rows(what: str, name: str, t: torch.Tensor, rows: int, cols: int) -> N
         raise KernelError(f"{what}: {name} must be 2-D with {rows} rows and {cols} columns next to one another")
 
 
+def _rows_overlap(a: torch.Tensor, b: torch.Tensor, rows: int, cols: int) -> bool:
+    """Whether the first ``rows`` x ``cols`` numbers of two matrices of one type have memory in common (columns next to one
+    another)."""
+    if rows <= 0 or cols <= 0:
+        return False
+    ahead, size = b.data_ptr() - a.data_ptr(), a.element_size()
+    if ahead < 0:
+        a, b, ahead = b, a, -ahead
+    step, width, last = a.stride(0) * size, cols * size, rows - 1
+    if ahead >= step * last + width:
+        return False
+    if last and step != b.stride(0) * size:
+        return True                                    # (rows that interleave unevenly: taken to meet)
+    if not last or step == 0:
+        return True
+    return ahead % step < width or ahead % step + width > step
+
+
 _E8, _U8, _I32, _F32T = torch.float8_e4m3fn, torch.uint8, torch.int32, torch.float32
 
 
@@ -1614,8 +1632,8 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
     """Attention of one new token per sequence over its rows of the 8-bit cache (its own key and value, at ``token_pos``,
     included): ``q`` [sequences, heads * head_dim] bfloat16 -> [sequences, heads * head_dim] bfloat16.  ``window``: as the other
     attention kernels take it (0: every key; w: keys t > pos - w; -c: chunks of c positions).  ``sink`` [heads] joins the
-    denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives NaN.  ``out`` is
-    another tensor than ``q``.  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
+    denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives NaN.  ``out`` has
+    no memory in common with ``q`` (columns of one buffer may).  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
     ``tickets`` (a zero int32 per sequence and chunk of 8 heads of a kv head, left zero) are made here when not given; given ones
     belong to one launch at a time.  Positions, slots and the page table are the step's inputs, which this kernel and the two above
     read while the package's kernel in front of them may still run: none of those writes them."""
@@ -1629,8 +1647,10 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
         out = torch.empty_like(q) if q.shape[1] == cols and q.is_contiguous() else q.new_empty((B, cols))
     else:
         _need_rows(what, "out", out, B, cols)
-        if B > 0 and out.data_ptr() == q.data_ptr():       # (one block writes a head while another has yet to read its query)
-            raise KernelError(f"{what}: out must be another tensor than q")
+        if B > 1 and out.stride(0) < cols:
+            raise KernelError(f"{what}: the rows of out overlap one another")
+        if _rows_overlap(out, q, B, cols):             # (one block writes a head while another has yet to read its query)
+            raise KernelError(f"{what}: out must be another tensor than q, with no memory in common")
     if seq_slot.numel() < B or token_pos.numel() < B:
         raise KernelError(f"{what}: a slot and a position per sequence")
     if sink is not None and sink.numel() != num_heads:

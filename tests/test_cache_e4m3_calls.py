@@ -51,3 +51,55 @@ def test_a_model_with_caches_of_both_kinds_hands_the_native_loop_what_each_needs
                   key_scales=torch.empty(1, dtype=torch.uint8) if e4m3 else None)
         run.run(model, torch.empty(tokens, d), ctx, NS(view=lambda i: view))
     assert seen == [(f"entry points {e}", e) for e in kinds]
+
+
+def _cache(hkv=2, hd=64, pages=3):
+    kp = torch.zeros(pages, hkv, 64, hd, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    sc = torch.zeros(pages, hkv, 64, dtype=torch.uint8)
+    return [kp, kp.clone(), sc, sc.clone(), torch.zeros(2, 4, dtype=torch.int32)]
+
+
+def _ints(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def test_decode_refuses_an_output_that_meets_the_queries_or_itself():
+    from dlgo_b200.csrc import kernels as K
+    cols = 256
+    buf = torch.zeros(4 * 3 * cols + 64, dtype=torch.bfloat16)
+
+    def rows(first, stride, n=3):
+        return buf.as_strided((n, cols), (stride, 1), first)
+
+    def decode(q, out):
+        return K.attention_decode_e4m3(q, *_cache(), _ints(*range(q.shape[0])), _ints(*[0] * q.shape[0]), 4, 2, 64, 1.0, out=out)
+
+    for q, out in ((rows(0, cols), rows(0, cols)), (rows(0, cols), rows(8, cols)), (rows(8, cols), rows(0, cols)),
+                   (rows(0, cols), rows(2 * cols, cols)), (rows(0, 2 * cols), rows(cols - 4, 2 * cols)),
+                   (rows(0, 2 * cols), rows(cols + 4, 2 * cols)), (rows(cols, 2 * cols), rows(0, cols)),
+                   (rows(0, cols, 1), rows(cols - 4, cols, 1)), (rows(0, 0), rows(0, cols))):
+        with pytest.raises(K.KernelError, match="another tensor"):
+            decode(q, out)
+    other = torch.zeros(3 * cols, dtype=torch.bfloat16)
+    for stride in (0, 4, cols - 4):
+        with pytest.raises(K.KernelError, match="overlap one another"):
+            decode(rows(0, cols), other.as_strided((3, cols), (stride, 1)))
+    # columns of one buffer, rows behind one another, more rows than sequences, one row: as before
+    for q, out in ((rows(0, 2 * cols), rows(cols, 2 * cols)), (rows(cols, 2 * cols), rows(0, 2 * cols)), (rows(0, cols), rows(3 * cols, cols)),
+                   (rows(3 * cols, cols, 2), rows(cols, cols, 4)[:3]), (rows(0, cols, 1), rows(cols, 0, 1)), (rows(0, 0), rows(cols, cols))):
+        with pytest.raises(K.KernelError, match="GPU"):
+            decode(q, out)
+
+
+def test_the_c_entry_refuses_rows_that_meet():
+    import struct
+
+    from dlgo_b200.csrc import kernels as K
+    fn = K._lib("attention_decode_e4m3").dlgo_attention_decode_e4m3_record
+
+    def call(B, ldq, ldo):        # (pointers are looked at for their alignment alone before the sizes are; B = 0 launches nothing)
+        p = 4096
+        return fn(struct.pack("=19qd4q", p, B, ldq, p, p, p, p, 3, p, 2, 4, p, p, p, ldo, 4, 2, 64, 0, 1.0, 0, p, p, 0))
+
+    assert K._STATUS[call(2, 256, 252)] == K._STATUS[call(2, 256, 0)] == K._STATUS[call(2, -256, 256)] == K._STATUS[call(2, 256, -256)]
+    assert "size" in K._STATUS[call(2, 256, 252)] and call(0, 256, 0) == 0
