@@ -1515,6 +1515,12 @@ def _rows_overlap(a: torch.Tensor, b: torch.Tensor, rows: int, cols: int) -> boo
     return ahead % step < width or ahead % step + width > step
 
 
+def _blocks_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors have memory in common."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
+
+
 _E8, _U8, _I32, _F32T = torch.float8_e4m3fn, torch.uint8, torch.int32, torch.float32
 
 
@@ -1553,7 +1559,7 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, to
     the tables are then not read), in pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1).  ``write_cache`` False:
     queries only (a layer that reads another's cache).  ``clear`` (fp32): zeros are left where ``qkv`` was read.  A position
     without a page, or of a sequence that ``seq_slot`` does not have, is not written (:func:`check_device_errors` reports it).  The tokens' positions are distinct within a
-    sequence."""
+    sequence, and keys and values lie in memory of their own."""
     what = "rope_append_e4m3"
     if num_heads <= 0 or num_kv_heads <= 0:
         raise KernelError(f"{what}: head counts must be positive")
@@ -1563,6 +1569,8 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, to
     if clear and code != F32:
         raise KernelError(f"{what}: only an fp32 sum can be cleared")
     _check_e4m3(what, kpages, vpages, kscales, vscales, page_table, num_kv_heads, head_dim)
+    if write_cache and (_blocks_overlap(kpages, vpages) or _blocks_overlap(kscales, vscales)):
+        raise KernelError(f"{what}: keys and values must be pages with no memory in common")
     if token_pos.numel() < T or token_seq.numel() < T or seq_slot.numel() == 0:
         raise KernelError(f"{what}: a position and a sequence per token, and a slot per sequence")
     if not 0 <= rotary_dim <= head_dim or rotary_dim % 2:
@@ -1590,7 +1598,7 @@ def read_pages_e4m3(kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.T
                     pages: torch.Tensor, keys: Optional[torch.Tensor] = None, values: Optional[torch.Tensor] = None) -> tuple:
     """Pages of the 8-bit cache as bfloat16 (exact): ``pages`` [n, 3] int32 lists (slot, page of its sequence, rows to read);
     returns (keys, values), each [n, kv heads, 64, head_dim], rows beyond the given number as zeros (a page that the table does
-    not have likewise).  ``keys`` / ``values``: buffers of that shape to fill instead of new ones."""
+    not have likewise).  ``keys`` / ``values``: buffers of that shape to fill instead of new ones, with no memory in common."""
     what = "read_pages_e4m3"
     _check_e4m3(what, kpages, vpages, kscales, vscales, page_table)
     if pages.dim() != 2 or pages.shape[1] != 3:
@@ -1600,6 +1608,8 @@ def read_pages_e4m3(kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.T
     for name, t in (("keys", keys), ("values", values)):
         if t is not None and tuple(t.shape) != shape:
             raise KernelError(f"{what}: {name} must be {shape}, is {tuple(t.shape)}")
+    if keys is not None and values is not None and _blocks_overlap(keys, values):
+        raise KernelError(f"{what}: keys and values must be buffers with no memory in common")
     keys = kpages.new_empty(shape, dtype=torch.bfloat16) if keys is None else keys
     values = torch.empty_like(keys) if values is None else values
     _need_e4m3(what, kpages.get_device(), ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),

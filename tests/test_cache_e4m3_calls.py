@@ -103,3 +103,30 @@ def test_the_c_entry_refuses_rows_that_meet():
 
     assert K._STATUS[call(2, 256, 252)] == K._STATUS[call(2, 256, 0)] == K._STATUS[call(2, -256, 256)] == K._STATUS[call(2, 256, -256)]
     assert "size" in K._STATUS[call(2, 256, 252)] and call(0, 256, 0) == 0
+
+
+def test_reading_into_one_buffer_and_writing_into_shared_pages_are_refused():
+    from dlgo_b200.csrc import kernels as K
+    cache = _cache()
+    buf = torch.zeros(2 * 2 * 64 * 64 + 8, dtype=torch.bfloat16)
+    one = lambda at: buf[at:at + 2 * 64 * 64].view(1, 2, 64, 64)  # noqa: E731
+    pages = torch.zeros(1, 3, dtype=torch.int32)
+    for a, b in ((0, 0), (0, 8), (8, 0), (0, 2 * 64 * 64 - 8)):
+        with pytest.raises(K.KernelError, match="in common"):
+            K.read_pages_e4m3(*cache, pages, one(a), one(b))
+    with pytest.raises(K.KernelError, match="GPU"):
+        K.read_pages_e4m3(*cache, pages, one(0), one(2 * 64 * 64))
+
+    def write(cache, **more):
+        cos = torch.zeros(10, 32)
+        return K.rope_append_e4m3(torch.zeros(1, 8 * 64), cos, cos, _ints(0), _ints(0), _ints(0), *cache, 4, 2, 64, 64, **more)
+
+    for i in (1, 3):
+        shared = list(cache)
+        shared[i] = shared[i - 1]
+        with pytest.raises(K.KernelError, match="in common"):
+            write(shared)
+        with pytest.raises(K.KernelError, match="GPU"):
+            write(shared, write_cache=False)
+    with pytest.raises(K.KernelError, match="GPU"):
+        write(cache)
