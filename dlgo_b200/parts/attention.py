@@ -109,8 +109,9 @@ class GQAAttention(Mixer):
         return -self.chunk if self.chunk else 0
 
     def takes_e4m3_cache(self) -> bool:
-        # (a subclass with a forward of its own appends to the cache itself)
-        return type(self).forward is GQAAttention.forward and K.e4m3_takes(self.head_dim, K.E4M3_PAGE)
+        # (a subclass with a forward of its own appends to the cache itself; one that keeps 16 bits of the softmax's weights would
+        # lose them: the 8-bit decode attention keeps 11, or 8 where a kv head has more than four query heads)
+        return type(self).forward is GQAAttention.forward and not self.split_weights and K.e4m3_takes(self.head_dim, K.E4M3_PAGE)
 
     # -------------------------------------------------------------------- forward
     def _decode_slices(self, T: int, pages: int, sms: int) -> tuple:

@@ -130,3 +130,13 @@ def test_reading_into_one_buffer_and_writing_into_shared_pages_are_refused():
             write(shared, write_cache=False)
     with pytest.raises(K.KernelError, match="GPU"):
         write(cache)
+
+
+def test_a_mixer_that_keeps_16_bits_of_its_weights_keeps_its_cache_too():
+    from dlgo_b200.parts.attention import GQAAttention
+    for heads in (4, 16):
+        mixer = GQAAttention(256, heads, 2, 64, 0.125)
+        assert mixer.takes_e4m3_cache()
+        mixer.split_weights = True
+        assert not mixer.takes_e4m3_cache()
+    assert not GQAAttention(256, 4, 2, 96, 0.125).takes_e4m3_cache()
