@@ -1549,14 +1549,14 @@ def _on_device_of(fn):
 
 
 @_on_device_of
-def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, token_pos: torch.Tensor, token_seq: torch.Tensor,
+def rope_append_e4m3(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], token_pos: torch.Tensor, token_seq: torch.Tensor,
                      seq_slot: torch.Tensor, kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.Tensor, vscales: torch.Tensor,
                      page_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, rotary_dim: int,
                      interleaved: bool = False, write_cache: bool = True, clear: bool = False) -> torch.Tensor:
     """Rotate the query and key heads of ``qkv`` [tokens, q | k | v columns] (fp32 or bfloat16) at their tokens' positions in
     fp32, store keys and values in the 8-bit pages of those positions, and return the queries [tokens, heads * head_dim] in
     bfloat16.  ``cos`` / ``sin`` [positions, rotary_dim / 2] fp32: the first ``rotary_dim`` numbers of a head are rotated (0: none;
-    the tables are then not read), in pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1).  ``write_cache`` False:
+    the tables are then not looked at and may be ``None``), in pairs (i, i + rotary_dim / 2) or, ``interleaved``, (2i, 2i + 1).  ``write_cache`` False:
     queries only (a layer that reads another's cache).  ``clear`` (fp32): zeros are left where ``qkv`` was read.  A position
     without a page, or of a sequence that ``seq_slot`` does not have, is not written (:func:`check_device_errors` reports it).  The tokens' positions are distinct within a
     sequence, and keys and values lie in memory of their own."""
@@ -1577,16 +1577,18 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, to
         raise KernelError(f"{what}: rotary_dim must be even and no more than {head_dim}")
     positions = 0
     if rotary_dim:
-        positions = cos.shape[0]
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != rotary_dim // 2 or positions == 0:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != rotary_dim // 2 or cos.shape[0] == 0:
             raise KernelError(f"{what}: cos and sin must be [positions, rotary_dim / 2]")
+        positions = cos.shape[0]
+    tables = (("cos", cos, _F32T), ("sin", sin, _F32T)) if rotary_dim else ()
     _need_e4m3(what, qkv.get_device(), ("kpages", kpages, _E8), ("vpages", vpages, _E8), ("kscales", kscales, _U8), ("vscales", vscales, _U8),
-               ("page_table", page_table, _I32), ("cos", cos, _F32T), ("sin", sin, _F32T), ("token_pos", token_pos, _I32),
-               ("token_seq", token_seq, _I32), ("seq_slot", seq_slot, _I32))
+               ("page_table", page_table, _I32), ("token_pos", token_pos, _I32), ("token_seq", token_seq, _I32), ("seq_slot", seq_slot, _I32),
+               *tables)
     q = qkv.new_empty((T, num_heads * head_dim), dtype=torch.bfloat16)      # (half the host time of torch.empty)
     st = _e4m3_entry("cache_e4m3", "dlgo_write_e4m3_record", "28q")(
-        qkv.data_ptr(), code, T, qkv.stride(0) if T > 1 else cols, cos.data_ptr(), sin.data_ptr(), positions, token_pos.data_ptr(),
-        token_seq.data_ptr(), seq_slot.data_ptr(), seq_slot.numel(), page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
+        qkv.data_ptr(), code, T, qkv.stride(0) if T > 1 else cols, cos.data_ptr() if tables else 0, sin.data_ptr() if tables else 0, positions,
+        token_pos.data_ptr(), token_seq.data_ptr(), seq_slot.data_ptr(), seq_slot.numel(), page_table.data_ptr(), page_table.shape[0],
+        page_table.shape[1],
         kpages.data_ptr(), vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(), kpages.shape[0], q.data_ptr(), num_heads, num_kv_heads, head_dim,
         rotary_dim, interleaved, write_cache, clear)
     _check(st, what, 1 if T > 0 else 0)

@@ -140,3 +140,17 @@ def test_a_mixer_that_keeps_16_bits_of_its_weights_keeps_its_cache_too():
         mixer.split_weights = True
         assert not mixer.takes_e4m3_cache()
     assert not GQAAttention(256, 4, 2, 96, 0.125).takes_e4m3_cache()
+
+
+def test_without_a_rotation_the_tables_are_not_looked_at():
+    from dlgo_b200.csrc import kernels as K
+
+    def write(cos, sin, rot):
+        return K.rope_append_e4m3(torch.zeros(1, 8 * 64), cos, sin, _ints(0), _ints(0), _ints(0), *_cache(), 4, 2, 64, rot)
+
+    for cos in (None, torch.zeros(0), torch.zeros(3, dtype=torch.float64)):
+        with pytest.raises(K.KernelError, match="GPU"):
+            write(cos, cos, 0)
+    for cos, sin in ((None, None), (torch.zeros(10, 32), None), (None, torch.zeros(10, 32)), (torch.zeros(32), torch.zeros(32))):
+        with pytest.raises(K.KernelError, match="cos and sin"):
+            write(cos, sin, 64)
