@@ -114,7 +114,7 @@ class Recorder:
     where another entry's are read)] in 64 bits.  Rows are read before pages are given back."""
 
     def __init__(self, engine):
-        self.cache = engine.cache
+        self.cache, self.entries = engine.cache, len(engine.model.order)
         self.taken, self.slots = [], {}
 
     def __enter__(self):
@@ -130,10 +130,8 @@ class Recorder:
         slot = self.plain[0]()
         n = self.cache.max_seq_len
         rows = []
-        for e in range(64):
+        for e in range(self.entries):
             view = self.cache.view(e)
-            if view is None:
-                break
             shape = (n, view.keys.shape[1], view.keys.shape[3])
             rows.append(tuple(torch.full(shape, float("nan"), dtype=torch.float64) for _ in range(2)) if view.writes else None)
         self.slots[slot] = dict(rows=rows, upto=0)
