@@ -184,13 +184,23 @@ struct DecPlace {
 // Shared memory: rings of keys and of values, two buffers of queries and of weights, scale bytes, barriers, ... , sequences
 template <int HD> constexpr int de_off_q = (DE_KST + DE_VST) * de_halves<HD> * 128 * HD;
 template <int HD> constexpr int de_off_p = de_off_q<HD> + 2 * 16 * HD;
-// (6 KB to spare with heads of 128: where 8 kv heads share 296 blocks, the 37 parts of a sequence are joined in one go)
-template <int HD> constexpr int de_off_sc = de_off_p<HD> + 2 * de_halves<HD> * 2048 + (HD == 128 ? 6144 : 0);
+// What lies behind the rings: scale bytes, barriers, maxima over the tile [2][4][GM] and, each per head, row scales, maxima and
+// sums; then the sequences.
+constexpr int DE_RED = 2 * 4 * DE_GM * 4, DE_MISC = 10 * DE_GM * 4 + 128;
+constexpr int de_seq_bytes(int B) { return (4 * B + 1) * 4; }
+template <int HD> constexpr int de_end_p = de_off_p<HD> + 2 * de_halves<HD> * 2048;
+template <int HD> constexpr int de_behind = DE_SC * de_halves<HD> * 256 + DE_BARS * 8 + DE_RED + DE_MISC + de_seq_bytes(DE_MAX_B);
+// A join holds its parts where the rings were, and behind them in all that DE_BLOCKS blocks leave of an SM's 228 KB (a block takes 1 KB
+// beside its own): what lies there is one go less where a sequence has a few parts more than the rings hold (37 parts of heads of
+// 128, 35 in the rings alone, 46 with this: one of 131,072 keys 46.3 us for 46.8; nowhere slower).
+template <int HD> constexpr int de_spare = (228 * 1024 / DE_BLOCKS - 1024 - de_end_p<HD> - de_behind<HD>) / 1024 * 1024;
+static_assert(de_spare<64> >= 0 && de_spare<128> >= 0, "the blocks of an SM fit");
+template <int HD> constexpr int de_off_sc = de_end_p<HD> + de_spare<HD>;
 template <int HD> constexpr int de_off_bars = de_off_sc<HD> + DE_SC * de_halves<HD> * 256;
-template <int HD> constexpr int de_off_red = de_off_bars<HD> + DE_BARS * 8;             // [2][4][GM] floats
-template <int HD> constexpr int de_off_misc = de_off_red<HD> + 2 * 4 * DE_GM * 4;    // row scales [2][GM], maxima and sums [GM][4], words
-template <int HD> constexpr int de_off_seq = de_off_misc<HD> + 10 * DE_GM * 4 + 128;
-template <int HD> constexpr size_t de_smem(int B) { return de_off_seq<HD> + (size_t)(4 * B + 1) * 4; }
+template <int HD> constexpr int de_off_red = de_off_bars<HD> + DE_BARS * 8;
+template <int HD> constexpr int de_off_misc = de_off_red<HD> + DE_RED;
+template <int HD> constexpr int de_off_seq = de_off_misc<HD> + DE_MISC;
+template <int HD> constexpr size_t de_smem(int B) { return de_off_seq<HD> + (size_t)de_seq_bytes(B); }
 
 template <int HD, int GM>
 __global__ void __launch_bounds__(DE_THREADS, DE_BLOCKS)

@@ -54,3 +54,15 @@ def test_decode_into_columns_beside_the_queries():
     want = K().attention_decode_e4m3(q, *args)
     K().attention_decode_e4m3(buf[:, :hq * hd], *args, out=buf[:, hq * hd:])
     assert torch.equal(buf[:, hq * hd:], want) and torch.equal(buf[:, :hq * hd], q)
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 8, 128), (7, 7, 128), (6, 6, 128), (36, 6, 128), (4, 4, 64), (3, 3, 64), (24, 3, 64), (42, 6, 64)])
+def test_decode_joins_about_as_many_parts_as_one_go_holds(hq, hkv, hd):
+    """One long sequence over all blocks of the device, 37 to 98 parts a kv head, around what shared memory holds at a time (45 to 91);
+    against a plain softmax in 64 bits with the tolerance of the other tests."""
+    import test_cache_e4m3_gpu as G
+    args, more, want = G._decode_case(hq, hkv, hd, [24000])
+    out = K().attention_decode_e4m3(*args, **more)
+    G._check_decode(out, want, hd, hq // hkv)
+    assert torch.equal(out, K().attention_decode_e4m3(*args, **more))
+    K().check_device_errors()
