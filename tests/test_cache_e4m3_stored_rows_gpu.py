@@ -68,3 +68,23 @@ def test_generation(name, mixed, how):
             ref = M.run(name, tuple(tokens), mixed, rows)[0][len(prompt) - 1:]
             behind = ref.amax(1) - ref[torch.arange(24), torch.tensor(out)]
             assert (behind <= 2 * 3e-2 * ref.abs().amax()).all(), (len(prompt), behind.tolist())
+
+
+OTHERS = {   # hidden, layers, ffn, heads, kv heads, head size, vocab
+    "inputs no multiple of eight": (100, 2, 260, 4, 2, 64, 300),
+    "sixteen query heads to one key head": (192, 2, 320, 16, 1, 64, 300),
+    "a key head each, a narrow model": (64, 2, 96, 5, 5, 128, 200),
+}
+
+
+@pytest.mark.parametrize("mixed", [False, True])
+@pytest.mark.parametrize("name", list(OTHERS))
+def test_other_sizes(name, mixed, monkeypatch):
+    """Contractions that run on the fp32 pipes, groups beyond one block's, prompts and single tokens in one step."""
+    from dlgo_b200.engine.engine import Engine
+    monkeypatch.setitem(E.SIZES, name, OTHERS[name])
+    spec = E.mixed_spec(name) if mixed else E.config(name).architecture_spec()
+    eng = Engine(spec=spec, tensors=dict(E.tensors(name)), max_tokens=1536, cache_dtype="e4m3")
+    eng.cache.poison()
+    _check_trace(eng, name, mixed, "batches")
+    _check_trace(eng, name, mixed, "pieces")
