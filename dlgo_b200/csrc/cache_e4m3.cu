@@ -172,8 +172,12 @@ __global__ void __launch_bounds__(WE_WARPS * 32) write_e4m3_kernel(WriteE8 p, in
 }
 
 // Any rotation: the first `rot` numbers of a head in either pairing, or none.  A warp per (token, head), HD / 32 numbers a
-// lane; a number's partner is read beside it.  Kept apart from the kernel above for its reach, not its speed: its accesses are
-// 4 to 16 bytes a lane and the cosines are read for every head again, but few layers rotate like that.
+// lane; a number's partner is read beside it.  Layers whose whole heads turn in neighbouring pairs take it for every token.
+//
+// Few tokens cost what they cost above: 8 of 32 + 2 * 8 heads of 64 1.3 us, 64 of 128 2.0 to 2.5.  From some hundred on it is bound by
+// its instructions (79 % of the issue slots, 9 % of the memory's rate): a warp's place, its position's page and the cosines are worked
+// out for 64 or 128 numbers alone.  From bfloat16, 32 + 2 * 8 heads of 64 in pairs: 1,300 tokens 17.3 us (split in halves, by the kernel
+// above: 4.7), 16,384 tokens 209 us, 13 % of the copy rate (35.5); heads of 128 240 us (63.7), half of each head turned 302.
 template <typename T, int HD>
 __global__ void __launch_bounds__(WE_WARPS * 32) write_e4m3_any_kernel(WriteE8 p) {
   pdl_launch_dependents();

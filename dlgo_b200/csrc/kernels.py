@@ -1515,12 +1515,6 @@ def _rows_overlap(a: torch.Tensor, b: torch.Tensor, rows: int, cols: int) -> boo
     return ahead % step < width or ahead % step + width > step
 
 
-def _blocks_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two contiguous tensors have memory in common."""
-    pa, pb = a.data_ptr(), b.data_ptr()
-    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
-
-
 _E8, _U8, _I32, _F32T = torch.float8_e4m3fn, torch.uint8, torch.int32, torch.float32
 
 
@@ -1569,7 +1563,8 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Option
     if clear and code != F32:
         raise KernelError(f"{what}: only an fp32 sum can be cleared")
     _check_e4m3(what, kpages, vpages, kscales, vscales, page_table, num_kv_heads, head_dim)
-    if write_cache and (_blocks_overlap(kpages, vpages) or _blocks_overlap(kscales, vscales)):
+    k_at, v_at, ks_at, vs_at, rows = kpages.data_ptr(), vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(), kscales.numel()
+    if write_cache and (abs(k_at - v_at) < rows * head_dim or abs(ks_at - vs_at) < rows):        # (a byte a number)
         raise KernelError(f"{what}: keys and values must be pages with no memory in common")
     if token_pos.numel() < T or token_seq.numel() < T or seq_slot.numel() == 0:
         raise KernelError(f"{what}: a position and a sequence per token, and a slot per sequence")
@@ -1589,7 +1584,7 @@ def rope_append_e4m3(qkv: torch.Tensor, cos: Optional[torch.Tensor], sin: Option
         qkv.data_ptr(), code, T, qkv.stride(0) if T > 1 else cols, cos.data_ptr() if tables else 0, sin.data_ptr() if tables else 0, positions,
         token_pos.data_ptr(), token_seq.data_ptr(), seq_slot.data_ptr(), seq_slot.numel(), page_table.data_ptr(), page_table.shape[0],
         page_table.shape[1],
-        kpages.data_ptr(), vpages.data_ptr(), kscales.data_ptr(), vscales.data_ptr(), kpages.shape[0], q.data_ptr(), num_heads, num_kv_heads, head_dim,
+        k_at, v_at, ks_at, vs_at, kpages.shape[0], q.data_ptr(), num_heads, num_kv_heads, head_dim,
         rotary_dim, interleaved, write_cache, clear)
     _check(st, what, 1 if T > 0 else 0)
     return q
@@ -1610,7 +1605,7 @@ def read_pages_e4m3(kpages: torch.Tensor, vpages: torch.Tensor, kscales: torch.T
     for name, t in (("keys", keys), ("values", values)):
         if t is not None and tuple(t.shape) != shape:
             raise KernelError(f"{what}: {name} must be {shape}, is {tuple(t.shape)}")
-    if keys is not None and values is not None and _blocks_overlap(keys, values):
+    if n > 0 and keys is not None and values is not None and abs(keys.data_ptr() - values.data_ptr()) < keys.numel() * keys.element_size():
         raise KernelError(f"{what}: keys and values must be buffers with no memory in common")
     keys = kpages.new_empty(shape, dtype=torch.bfloat16) if keys is None else keys
     values = torch.empty_like(keys) if values is None else values
