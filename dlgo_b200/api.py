@@ -191,7 +191,8 @@ def load_llm(model_path: str, max_seq_len: int = 0, *, dtype: str = "bfloat16", 
     reference's ``LoadLLM(path, maxSeqLen)`` (dlgo.go:37-48).  ``max_tokens`` sizes the
     cache: positions that live sequences may hold together (default: ``max_batch``
     sequences of ``max_seq_len``, within half of the device's free memory).  ``cache_dtype="e4m3"`` keeps
-    keys and values in 8 bits: half the bytes to hold and to read for every token.
+    keys and values in 8 bits: half the bytes to hold and to read for every token, for slower prompts
+    (:class:`Engine` says when it pays).
     """
     engine = Engine(model_path, dtype=dtype, device=device, max_tokens=max_tokens,
                     max_seq_len=max_seq_len if max_seq_len > 0 else None, cuda_graphs=cuda_graphs,

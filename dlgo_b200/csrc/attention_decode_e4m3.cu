@@ -17,7 +17,9 @@
 // the first leaves over is at most 2^-4 of it); a weight as w1 + w2 / 16, 2^-8 of its size, or, where a block has four heads at
 // most and columns are left, + w3 / 256, 2^-11 (it passes through float16); and 2^-22 (2^-26) of the tile's largest weight.
 // The values' powers are part of the weights, so a row of small values may hold all of the softmax's weight without a loss;
-// and because every tile has a reference of its own, neither does a long tail of small weights behind a large one.
+// and because every tile has a reference of its own, neither does a long tail of small weights behind a large one.  s_j + b_j is one
+// 32-bit number: a result is off by 2^-24 |s_j| relative to itself (as far as a score's own sum is), and what scores below -1e30 counts
+// as not seen.
 //
 // Bound by the rows, which are read once.  The keys (of the scores) and the numbers of a head (of the output) are the
 // MMA's rows and the query heads of a kv head, times their terms, its 16 columns, so no thread touches a row: per tile

@@ -59,7 +59,9 @@ class Engine:
         (models/llm/generate.go:56-58).  ``max_slots``: sequences that may be live at once (default:
         one per page of the cache, but no more than keep a group's page table within 64 MB).
         ``cache_dtype``: ``"e4m3"`` keeps keys and values in 8 bits, a power of two per row of a head beside them: half the bytes
-        per position, for bfloat16 runs whose layers are grouped-query attention with heads of 64 or 128 (default: ``dtype``).
+        per position, for bfloat16 runs whose layers are grouped-query attention with heads of 64 or 128 (default: ``dtype``).  Large
+        batches and long sequences decode faster for it; one short sequence, prompts, and steps that bring prompts and single tokens
+        together take longer (their rows are read back as bfloat16 first).
 
         A model comes from ``model_dir`` (config.json chooses the architecture), or from an
         :class:`ArchitectureSpec` and its tensors given in memory (``spec``, ``tensors``)."""
