@@ -1639,8 +1639,10 @@ def attention_decode_e4m3(q: torch.Tensor, kpages: torch.Tensor, vpages: torch.T
     """Attention of one new token per sequence over its rows of the 8-bit cache (its own key and value, at ``token_pos``,
     included): ``q`` [sequences, heads * head_dim] bfloat16 -> [sequences, heads * head_dim] bfloat16.  ``window``: as the other
     attention kernels take it (0: every key; w: keys t > pos - w; -c: chunks of c positions).  ``sink`` [heads] joins the
-    denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives NaN.  ``out`` has
-    no memory in common with ``q`` (columns of one buffer may).  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
+    denominator.  A position of -1 sees nothing and gives zeros; a query head with an infinity or a NaN gives NaN.  A weight of
+    the softmax, times its value's power of two, is held to 11 bits (8 where a kv head has more than four query heads) and to 2^-26 (2^-22)
+    of the largest one of its 128 or 256 keys, a query's number to 2^-22 of its head's largest; everything else in 32 bits.
+    ``out`` has no memory in common with ``q`` (columns of one buffer may).  ``scratch`` (:func:`attention_decode_e4m3_scratch` floats) and
     ``tickets`` (a zero int32 per sequence and chunk of 8 heads of a kv head, left zero) are made here when not given; given ones
     belong to one launch at a time.  Positions, slots and the page table are the step's inputs, which this kernel and the two above
     read while the package's kernel in front of them may still run: none of those writes them."""

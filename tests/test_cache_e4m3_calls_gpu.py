@@ -66,3 +66,39 @@ def test_decode_joins_about_as_many_parts_as_one_go_holds(hq, hkv, hd):
     G._check_decode(out, want, hd, hq // hkv)
     assert torch.equal(out, K().attention_decode_e4m3(*args, **more))
     K().check_device_errors()
+
+
+def _off_by(args, more, lens, want, out, hd, group):
+    """The largest error over its bound.  As in the other tests, with the bound of what is lost below the smallest term of a weight
+    written out: 2^-22 of the largest weight of a tile (2^-26 with three terms), a weight being a softmax's times its value's power
+    of two, for every number that the values hold.  It matters where the heaviest key's value is zero at a number and a key far
+    lighter is all that is left there.  (Weights counted against the whole row's largest: no less than a tile's.)"""
+    import plain_e4m3 as P
+    hq, hkv, scale, worst = args[8], args[9], args[11], 0.0
+    pages, table, slots = [a.cpu() for a in args[1:5]], args[5].cpu(), args[6].tolist()
+    for i, (o, pv, mass, most) in enumerate(want):
+        n = lens[i]
+        at = table[slots[i], :-(-n // 64)].long()
+        k, v = (P.values(pages[j][at], pages[j + 2][at]).transpose(1, 2).reshape(-1, hkv, hd)[:n] for j in (0, 1))
+        power = P.two_to(pages[3][at].transpose(1, 2).reshape(-1, hkv)[:n].long() - 127)
+        s = torch.einsum("hd,nhd->hn", args[0][i].cpu().double().view(hq, hd), k.repeat_interleave(group, 1)) * scale
+        if more["sink"] is not None:
+            s = torch.cat([s, more["sink"].cpu().double().view(-1, 1)], 1)
+        p = torch.softmax(s, 1)[:, :n]
+        weight, least = (2.0 ** -11, 2.0 ** -26) if group <= 4 else (2.0 ** -8, 2.0 ** -22)
+        lost = least * (p * power.repeat_interleave(group, 1).T).amax(1, keepdim=True) * (v / power.unsqueeze(-1)).abs().sum(0).repeat_interleave(group, 0)
+        tol = 2.0 ** -8 * o.abs() + (weight + 2.0 ** -20 + (2 * (hd + 8) * 2.0 ** -24 + hd * 2.0 ** -22) * 1.5 * mass) * pv
+        tol = tol + lost * (1 + 2.0 ** -8) + 2.0 ** -134 + 2.0 ** -126 * most
+        worst = max(worst, float(((out[i].cpu().double().view(o.shape) - o).abs() / tol).max()))
+    return worst
+
+
+@pytest.mark.parametrize("hq,hkv,hd", [(6, 2, 64), (16, 1, 128), (45, 5, 128), (24, 1, 64), (8, 8, 128)])
+@pytest.mark.parametrize("lens", [[1 + i % 3 for i in range(40)], [6, 20, 2, 1, 27, 3], [1 + 7 * i % 31 for i in range(150)]])
+@pytest.mark.parametrize("shape", ["_sharp", "_tiny_and_huge"])
+def test_decode_of_few_keys_whose_weights_are_far_apart(hq, hkv, hd, lens, shape):
+    import test_cache_e4m3_gpu as G
+    for sink in (False, True):
+        args, more, want = G._decode_case(hq, hkv, hd, lens, sink=sink, shape=getattr(G, shape))
+        out = K().attention_decode_e4m3(*args, **more)
+        assert _off_by(args, more, lens, want, out, hd, hq // hkv) <= 1
