@@ -1506,13 +1506,14 @@ def _rows_overlap(a: torch.Tensor, b: torch.Tensor, rows: int, cols: int) -> boo
     if ahead < 0:
         a, b, ahead = b, a, -ahead
     step, width, last = a.stride(0) * size, cols * size, rows - 1
-    if ahead >= step * last + width:
-        return False
-    if last and step != b.stride(0) * size:
-        return True                                    # (rows that interleave unevenly: taken to meet)
-    if not last or step == 0:
-        return True
-    return ahead % step < width or ahead % step + width > step
+    step_b = b.stride(0) * size
+    for at in range(ahead, ahead + (step_b * last if step_b != step else 0) + 1, max(step_b, 1)):     # (rows of b; of equal strides the first)
+        if at >= step * last + width:
+            break
+        row, inside = divmod(at, step) if last and step else (0, at)
+        if inside < width or (row < last and inside + width > step):
+            return True
+    return False
 
 
 _E8, _U8, _I32, _F32T = torch.float8_e4m3fn, torch.uint8, torch.int32, torch.float32

@@ -154,3 +154,23 @@ def test_without_a_rotation_the_tables_are_not_looked_at():
     for cos, sin in ((None, None), (torch.zeros(10, 32), None), (None, torch.zeros(10, 32)), (torch.zeros(32), torch.zeros(32))):
         with pytest.raises(K.KernelError, match="cos and sin"):
             write(cos, sin, 64)
+
+
+def test_overlap_of_rows_agrees_with_a_count_of_their_numbers():
+    import random
+
+    from dlgo_b200.csrc import kernels as K
+    rng = random.Random(0)
+    buf = torch.zeros(400, dtype=torch.bfloat16)
+    seen = [0, 0]
+    for _ in range(4000):
+        rows, cols = rng.randint(1, 5), rng.randint(1, 12)
+        a, b = (dict(first=rng.randint(0, 90), stride=rng.choice([0, cols, rng.randint(0, 60), 24])) for _ in range(2))
+        if rng.random() < 0.5:
+            b["stride"] = a["stride"]
+        numbers = [{t["first"] + r * t["stride"] + c for r in range(rows) for c in range(cols)} for t in (a, b)]
+        want = bool(numbers[0] & numbers[1])
+        x, y = (buf.as_strided((rows, cols), (t["stride"], 1), t["first"]) for t in (a, b))
+        assert K._rows_overlap(x, y, rows, cols) == K._rows_overlap(y, x, rows, cols) == want, (rows, cols, a, b)
+        seen[want] += 1
+    assert min(seen) > 500
